@@ -386,6 +386,56 @@ int mi355_paged_attn_rows_ragged(const void* q, const mi355_kv_layer_t* kv, cons
                                  int32_t rows, int32_t nh, float scale, int32_t max_seq_len, void* out, void* workspace,
                                  size_t workspace_bytes, mi355_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * A paged cache whose slots are not positions, attention with score forms over it, and eviction by attention weight.
+ *
+ * Two planes beside the cache, indexed as its scale plane is, [num_blocks][nkv][page]: key_pos (int32, the position of the token in a slot, per kv head,
+ * as heads may keep different tokens) and weights (fp32, the attention weight that the token has drawn).  Pages of a sequence that is tracked or evicted are its own.
+ *
+ * mi355_rope_kv_write_slots: mi355_rope_kv_write_rows for 16-bit rows (row_seq null: row t is of sequence t / q_len, T = nseq q_len; else of row_seq[t] and q_len is 1) whose
+ *   rotation goes by positions[t] (cos_sin null: no rotation, any position >= 0) and whose K / V are stored at slot slots[t] of the sequence; slots[t] < 0: a padding row.  The
+ *   position goes to key_pos and 0 to weights there (either may be null).  A row whose position, slot, sequence or block id is out of range is not stored and counted once in oob_count.
+ */
+int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias, const float* cos_sin, int32_t max_pos, const int32_t* positions,
+                              const int32_t* slots, const int32_t* row_seq, const int32_t* block_table, int32_t max_blocks_per_seq, int32_t nseq, int32_t T,
+                              int32_t q_len, int32_t nh, const mi355_kv_layer_t* kv, void* q_out, int32_t* key_pos, float* weights, int32_t* oob_count,
+                              mi355_stream_t stream);
+
+/* mi355_paged_attn_scored: rows of attention over the paged cache, of one or many rows a sequence, whose scores have a form:
+ *     u = scale q.k;   s = softcap > 0 ? softcap tanh(u / softcap) : u;   with slopes: s += slopes[h] (key position - positions[row]),
+ *   the key position from key_pos, or the slot itself where that is null.  Row r sees the slots begin[r] .. end[r] - 1 of its sequence (begin null: from 0; end is clamped to
+ *   max_seq_len): causal rows have end = slot + 1, a window begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = the document's
+ *   first slot.  A row that sees nothing gets zeros and a log-sum-exp of -inf.  Block ids are clamped into the pool; what slots that no row of a sequence sees hold, NaN
+ *   included, does not matter.
+ *   q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows behind the last are left alone), or, row_start null,
+ *   b q_len .. and rows = B q_len.  out [rows][nh hd]; lse [rows][nh] (fp32, natural logarithm) or null.  Any number of heads per kv head.
+ *   weights (plane, or null): for every slot below the largest end of its sequence's rows that see something, weights <- decay weights + the sum over the sequence's rows and the heads of the
+ *   kv head of exp(s - lse) (decay 1: accumulated since the start; 0: the last call's alone, whatever was there; between: fading).
+ *   workspace: as many bytes as mi355_paged_attn_scored_workspace_bytes says, on 16 bytes; calls that may overlap need their own. */
+typedef struct {
+    float          scale, softcap;
+    const float*   slopes;     /* dev [nh] or NULL */
+    const int32_t* positions;  /* dev [rows], with slopes */
+    const int32_t* key_pos;    /* dev plane or NULL */
+    const int32_t* begin;      /* dev [rows] or NULL */
+    const int32_t* end;        /* dev [rows] */
+} mi355_attn_score_t;
+size_t mi355_paged_attn_scored_workspace_bytes(int32_t B, int32_t q_len, int32_t rows, int32_t nh, int32_t nkv, int32_t hd, int32_t max_seq_len, int32_t track);
+int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_kv_layer_t* kv, const int32_t* block_table, int32_t max_blocks_per_seq,
+                            const int32_t* row_start, int32_t B, int32_t q_len, int32_t rows, int32_t nh, const mi355_attn_score_t* score,
+                            int32_t max_seq_len, void* out, float* lse, float* weights, float decay, void* workspace, size_t workspace_bytes,
+                            mi355_stream_t stream);
+
+/* mi355_kv_evict: every (sequence, kv head) with more than `keep` tokens keeps `keep` of them: those at positions < sinks or >= next_pos[b] - recent first (sinks + recent <= keep),
+ *   then the ones with the largest weights, the lower slot where weights are equal (NaN counts as the smallest).  Kept tokens in slots below `keep` stay where they are; the i-th of those
+ *   behind moves into the i-th slot that an evicted token leaves: keys, values, scales, weights and positions.  What lies in slots >= keep afterwards is unspecified but still the pool's.
+ *   new_lens[b] = min(seq_lens[b], keep) (may be null or seq_lens).  seq_lens are clamped to [0, max_seq_len]; tokens in blocks outside the pool are the first to go and never moved.
+ *   The caller appends at slot new_lens[b] and may free the pages behind it. */
+size_t mi355_kv_evict_workspace_bytes(int32_t B, int32_t nkv, int32_t keep, int32_t max_seq_len);
+int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_t* key_pos, const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* seq_lens,
+                   const int32_t* next_pos, int32_t B, int32_t max_seq_len, int32_t keep, int32_t sinks, int32_t recent, int32_t* new_lens, void* workspace,
+                   size_t workspace_bytes, mi355_stream_t stream);
+
 /* Greedy fast path: ids[b] = argmax(logits[b, :]) on fp32 logits, lowest index on ties
  * (bindings/core/CudaSampleOp.cc:687-700).  workspace >= B * 64 * 8 bytes. */
 int mi355_argmax(const float* logits, int32_t B, int32_t V, int32_t ld, int32_t* ids,

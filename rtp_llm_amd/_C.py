@@ -35,6 +35,10 @@ class KVLayer(C.Structure):  # mi355_kv_layer_t
                 ("nkv", i32), ("hd", i32), ("num_blocks", i32), ("act_dtype", i32)]
 
 
+class AttnScore(C.Structure):  # mi355_attn_score_t
+    _fields_ = [("scale", f32), ("softcap", f32), ("slopes", vp), ("positions", vp), ("key_pos", vp), ("begin", vp), ("end", vp)]
+
+
 class FusedNorm(C.Structure):  # mi355_fused_norm_t
     _fields_ = [("tile_sumsq", vp), ("tiles", i32), ("ld", i32), ("weight", vp), ("eps", f32)]
 
@@ -133,6 +137,11 @@ SIGNATURES = {
     "mi355_rope_kv_write_rows_ragged": (i32, [vp, vp, i32, i32, vp, vp, i32, i32, vp, vp, vp, i32, i32, i32, i32, C.POINTER(KVLayer), vp, vp, vp]),
     "mi355_paged_attn_rows_ragged": (i32, [vp, C.POINTER(KVLayer), vp, i32, vp, vp, i32, i32, i32, i32, f32, i32, vp, vp, sz, vp]),
     "mi355_paged_attn_rows": (i32, [vp, C.POINTER(KVLayer), vp, i32, vp, i32, i32, i32, f32, i32, vp, vp, sz, vp]),
+    "mi355_rope_kv_write_slots": (i32, [vp, i32, vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, C.POINTER(KVLayer), vp, vp, vp, vp, vp]),
+    "mi355_paged_attn_scored_workspace_bytes": (sz, [i32] * 8),
+    "mi355_paged_attn_scored": (i32, [vp, i32, C.POINTER(KVLayer), vp, i32, vp, i32, i32, i32, i32, C.POINTER(AttnScore), i32, vp, vp, vp, f32, vp, sz, vp]),
+    "mi355_kv_evict_workspace_bytes": (sz, [i32] * 4),
+    "mi355_kv_evict": (i32, [C.POINTER(KVLayer), vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, vp, vp, sz, vp]),
     "mi355_argmax": (i32, [vp, i32, i32, i32, vp, vp, sz, vp]),
     "mi355_sampling_probs_workspace_bytes": (sz, [i32]),
     "mi355_sampling_probs": (i32, [vp, i32, i32, i32, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, vp, vp]),

@@ -29,10 +29,33 @@ struct RopeParams {
     float*         scale_base;
     int            kv_int8;
     f16*           q_out;
+    // SLOTS instances (mi355_rope_kv_write_slots): the row is rotated at its position (cos_sin null: not at all) and stored at a slot of its own
+    const int32_t* slots;
+    int            nseq;
+    int32_t*       key_pos;   // nullable [blocks][nkv][page]: receives the position
+    float*         weights;   // nullable, the same: receives 0
 };
+// where row t is stored: the slot asked for, and whether its position can be rotated and kept
+template <bool SLOTS> struct RopePlace { int pos_in, pos, slot_in, slot, seq; };
+template <bool SLOTS> __device__ __forceinline__ RopePlace<SLOTS> rope_place(const RopeParams& p, int t) {
+    RopePlace<SLOTS> r;
+    r.pos_in = p.positions[t];
+    r.seq = p.row_seq ? p.row_seq[t] : t / p.q_len;
+    if constexpr (SLOTS) {
+        r.pos = min(max(r.pos_in, 0), p.max_pos - 1);
+        r.slot_in = p.slots[t];
+        r.slot = min(max(r.slot_in, 0), p.max_blocks * p.page - 1);
+        if ((unsigned)r.seq >= (unsigned)p.nseq) { r.seq = 0; if (r.slot_in >= 0) r.slot_in = 0x7fffffff; }   // no such sequence: as a slot out of range
+    } else {
+        const int pos_lim = min(p.max_pos, p.max_blocks * p.page);
+        r.pos = min(max(r.pos_in, 0), pos_lim - 1);       // clamped: the rotation table and the block table stay in range
+        r.slot_in = r.pos_in; r.slot = r.pos;
+    }
+    return r;
+}
 
 // BF: qkv / bias / q_out and a 16-bit cache are bf16 (kv_dtype MI355_KV_BF16); the INT8 cache is quantised from the same fp32 values either way
-template <bool BF>
+template <bool BF, bool SLOTS>
 __global__ __launch_bounds__(256) void rope_kv_write_kernel(const RopeParams p) {
     using raw16 = uint16_t;
     const int t    = blockIdx.x;
@@ -47,13 +70,11 @@ __global__ __launch_bounds__(256) void rope_kv_write_kernel(const RopeParams p) 
     // Everything is requested before the first wait (round 2 walked 8 dependent round trips: 4 slabs, 3 tail slabs one by
     // one, bias, position, rotation row, block id): the position and the block id are wave-uniform (scalar loads), the
     // slabs of a column are up to 16 independent loads, the rotation row follows the position.
-    const int pos_in = p.positions[t];
-    const int pos_lim = min(p.max_pos, p.max_blocks * p.page);
-    const int pos = min(max(pos_in, 0), pos_lim - 1);       // clamped: the rotation table and the block table stay in range
+    const RopePlace<SLOTS> at = rope_place<SLOTS>(p, t);
     const bool is_v = h >= p.nh + p.nkv;
-    const int blk = (h >= p.nh) ? p.block_table[(size_t)(p.row_seq ? p.row_seq[t] : t / p.q_len) * p.max_blocks + pos / p.page] : 0;
+    const int blk = (h >= p.nh) ? p.block_table[(size_t)at.seq * p.max_blocks + at.slot / p.page] : 0;
     float2 cs = {1.f, 0.f};
-    if (!is_v && act) cs = *reinterpret_cast<const float2*>(p.cos_sin + ((size_t)pos * half + lane) * 2);
+    if (!is_v && act && (!SLOTS || p.cos_sin)) cs = *reinterpret_cast<const float2*>(p.cos_sin + ((size_t)at.pos * half + lane) * 2);
     float x0 = 0.f, x1 = 0.f;
     if (act) {
         float bh0 = 0.f, bh1 = 0.f;
@@ -96,12 +117,16 @@ __global__ __launch_bounds__(256) void rope_kv_write_kernel(const RopeParams p) 
     }
     // ---- K / V into the paged cache
     const int kh  = is_v ? h - p.nh - p.nkv : h - p.nh;
-    if (pos_in < 0) return;                                  // padding row of a multi-row step: nothing to store
-    if (pos != pos_in || blk < 0 || blk >= p.num_blocks) {   // stale position / block id: never write somebody else's page
+    if (at.slot_in < 0) return;                              // padding row of a multi-row step: nothing to store
+    if (at.pos != at.pos_in || at.slot != at.slot_in || blk < 0 || blk >= p.num_blocks) {   // stale position / block id: never write somebody else's page
         if (h == p.nh && lane == 0 && p.oob_count) atomicAdd(p.oob_count, 1);
         return;
     }
-    const int tok = pos % p.page;
+    const int tok = at.slot % p.page;
+    if constexpr (SLOTS) {
+        const size_t plane = ((size_t)blk * p.nkv + kh) * p.page + tok;
+        if (!is_v && lane == 0) { if (p.key_pos) p.key_pos[plane] = at.pos; if (p.weights) p.weights[plane] = 0.f; }
+    }
     const size_t head_elems = (size_t)p.page * p.hd;
     const size_t blk_base   = ((size_t)blk * 2 + (is_v ? 1 : 0)) * p.nkv + kh; // in units of heads
     int s0, s1; // element offsets inside this head's [page*hd] region
@@ -133,12 +158,11 @@ __global__ __launch_bounds__(256) void rope_kv_write_kernel(const RopeParams p) 
 // consecutive rows from eight L2s.  us by waves / here: 28 over 4 heads of 128, 4096 rows 31.7 / 15.9
 // (4.7 TB/s), 1055 10.5 / 6.6, 265 4.5 / 4.2; 14 over 2 of 64, 4096 15.7 / 6.1, 512 4.1 / 3.2; 32 over 32 of 64, 1055 25.8 / 8.6, 64 3.8 / 3.0.
 constexpr int RP_ROWS = 16, RP_HEADS = 4;
-template <bool BF, int HD>
+template <bool BF, int HD, bool SLOTS>
 __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p) {
     constexpr int half = HD / 2, P = half / 8, LD = HD + 2;                  // 16-byte pieces of a half, a row of values in LDS
     __shared__ uint32_t vs[RP_ROWS * LD / 2];
     const int t0 = blockIdx.x * RP_ROWS, nrot = p.nh + p.nkv, chunks = (nrot + RP_HEADS - 1) / RP_HEADS;
-    const int pos_lim = min(p.max_pos, p.max_blocks * p.page);
     const uint16_t* qkv = reinterpret_cast<const uint16_t*>(p.qkv);
     const uint16_t* bias = reinterpret_cast<const uint16_t*>(p.bias);
     auto load8 = [&](int t, int col, float (&x)[8]) {                        // a row's 8 columns with their bias, rounded
@@ -148,11 +172,11 @@ __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) { x[2 * i] = act_round<BF>(act_lo<BF>(v[i]) + act_lo<BF>(b[i])); x[2 * i + 1] = act_round<BF>(act_hi<BF>(v[i]) + act_hi<BF>(b[i])); }
     };
-    auto place = [&](int t, int pos_in, int pos, size_t heads, uint16_t*& dst, int& tok) -> int {     // the page of a row (heads: units of heads behind a block's first): 0 none, -1 out of range
-        if (pos_in < 0) return 0;
-        const int blk = p.block_table[(size_t)(p.row_seq ? p.row_seq[t] : t / p.q_len) * p.max_blocks + pos / p.page];
-        if (pos != pos_in || blk < 0 || blk >= p.num_blocks) return -1;
-        tok = pos % p.page;
+    auto place = [&](int t, const RopePlace<SLOTS>& at, size_t heads, uint16_t*& dst, int& tok, int& blk) -> int {     // the page of a row (heads: units of heads behind a block's first): 0 none, -1 out of range
+        if (at.slot_in < 0) return 0;
+        blk = p.block_table[(size_t)at.seq * p.max_blocks + at.slot / p.page];
+        if (at.pos != at.pos_in || at.slot != at.slot_in || blk < 0 || blk >= p.num_blocks) return -1;
+        tok = at.slot % p.page;
         dst = (uint16_t*)p.kv_base + ((size_t)blk * 2 * p.nkv + heads) * p.page * HD;
         return 1;
     };
@@ -161,13 +185,13 @@ __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p)
         for (int i = 0; i < RP_ROWS * RP_HEADS * P / 256; ++i) {
             const int item = i * 256 + (int)threadIdx.x, c = item % P * 8, h = blockIdx.y * RP_HEADS + item / P % RP_HEADS, t = t0 + item / (P * RP_HEADS);
             if (h >= nrot || t >= p.T) continue;
-            const int pos_in = p.positions[t], pos = min(max(pos_in, 0), pos_lim - 1);
+            const RopePlace<SLOTS> where = rope_place<SLOTS>(p, t);
             float x0[8], x1[8];
             load8(t, h * HD + c, x0); load8(t, h * HD + half + c, x1);
-            const float4* rot = reinterpret_cast<const float4*>(p.cos_sin + ((size_t)pos * half + c) * 2);
+            const float4* rot = reinterpret_cast<const float4*>(p.cos_sin + ((size_t)where.pos * half + c) * 2);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float4 cs = rot[k];
+                const float4 cs = !SLOTS || p.cos_sin ? rot[k] : make_float4(1.f, 0.f, 1.f, 0.f);
                 const float a0 = x0[2 * k], b0 = x1[2 * k], a1 = x0[2 * k + 1], b1 = x1[2 * k + 1];
                 x0[2 * k] = cs.x * a0 - cs.y * b0; x1[2 * k] = cs.x * b0 + cs.y * a0;
                 x0[2 * k + 1] = cs.z * a1 - cs.w * b1; x1[2 * k + 1] = cs.z * b1 + cs.w * a1;
@@ -178,10 +202,16 @@ __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p)
             uint16_t* dst;
             if (h < p.nh) dst = reinterpret_cast<uint16_t*>(p.q_out) + ((size_t)t * p.nh + h) * HD + c;
             else {
-                int tok = 0;
-                const int at = place(t, pos_in, pos, h - p.nh, dst, tok);
+                int tok = 0, blk;
+                const int at = place(t, where, h - p.nh, dst, tok, blk);
                 if (at < 0 && h == p.nh && c == 0 && p.oob_count) atomicAdd(p.oob_count, 1);
                 if (at <= 0) continue;
+                if constexpr (SLOTS)
+                    if (c == 0) {
+                        const size_t plane = ((size_t)blk * p.nkv + h - p.nh) * p.page + tok;
+                        if (p.key_pos) p.key_pos[plane] = where.pos;
+                        if (p.weights) p.weights[plane] = 0.f;
+                    }
                 dst += tok * HD + c;
             }
             *reinterpret_cast<u32x4*>(dst) = y0;
@@ -201,10 +231,9 @@ __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p)
     __syncthreads();
     const int r = threadIdx.x % RP_ROWS, t = t0 + r;
     if (t >= p.T) return;
-    const int pos_in = p.positions[t];
     uint16_t* dst;
-    int tok = 0;
-    if (place(t, pos_in, min(max(pos_in, 0), pos_lim - 1), p.nkv + kh, dst, tok) <= 0) return;
+    int tok = 0, blk;
+    if (place(t, rope_place<SLOTS>(p, t), p.nkv + kh, dst, tok, blk) <= 0) return;
     for (int d = threadIdx.x / RP_ROWS; d < HD; d += 256 / RP_ROWS) dst[(size_t)d * p.page + tok] = reinterpret_cast<const uint16_t*>(vs)[r * LD + d];
 }
 
@@ -228,15 +257,16 @@ extern "C" int mi355_rope_kv_write_rows(const void* qkv_f16, const float* partia
                                            max_blocks_per_seq, T, q_len, nh, kv, q_out, oob_count, stream);
 }
 
-// row_seq non-null (device, [T]): the sequence of every row; q_len is 1 then
-extern "C" int mi355_rope_kv_write_rows_ragged(const void* qkv_f16, const float* partials, int32_t nsplit, int32_t ld,
-                                               const void* qkv_bias, const float* cos_sin, int32_t rope_dim, int32_t max_pos,
-                                               const int32_t* positions, const int32_t* row_seq, const int32_t* block_table, int32_t max_blocks_per_seq,
-                                               int32_t T, int32_t q_len, int32_t nh, const mi355_kv_layer_t* kv, void* q_out,
-                                               int32_t* oob_count, mi355_stream_t stream) {
+namespace {
+struct RopeSlots { const int32_t* slots; int nseq; int32_t* key_pos; float* weights; };
+
+template <bool SLOTS>
+int launch_rope(const void* qkv_f16, const float* partials, int32_t nsplit, int32_t ld, const void* qkv_bias, const float* cos_sin, int32_t rope_dim, int32_t max_pos,
+                const int32_t* positions, const int32_t* row_seq, const int32_t* block_table, int32_t max_blocks_per_seq, int32_t T, int32_t q_len, int32_t nh,
+                const mi355_kv_layer_t* kv, void* q_out, int32_t* oob_count, const RopeSlots& to, mi355_stream_t stream) {
     MI355_CHECK_ARG(q_len >= 1 && T % q_len == 0, "rope_kv_write: T=%d must be a multiple of q_len=%d", T, q_len);
     MI355_CHECK_ARG((qkv_f16 != nullptr) != (partials != nullptr), "rope_kv_write: exactly one of qkv_f16 / partials");
-    MI355_CHECK_ARG(kv && kv->kv_base && cos_sin && positions && block_table && q_out, "rope_kv_write: null pointer");
+    MI355_CHECK_ARG(kv && kv->kv_base && (cos_sin || SLOTS) && positions && block_table && q_out, "rope_kv_write: null pointer");
     MI355_CHECK_ARG(kv->hd == 64 || kv->hd == 128, "rope_kv_write: hd=%d (64 or 128)", kv->hd);
     MI355_CHECK_ARG(rope_dim == kv->hd, "rope_kv_write: rope_dim=%d must equal hd=%d", rope_dim, kv->hd);
     MI355_CHECK_ARG(kv->page > 0 && T > 0 && nh > 0 && kv->nkv > 0 && max_pos > 0 && max_blocks_per_seq > 0 && kv->num_blocks > 0,
@@ -254,23 +284,45 @@ extern "C" int mi355_rope_kv_write_rows_ragged(const void* qkv_f16, const float*
     p.T = T; p.nh = nh; p.nkv = kv->nkv; p.hd = kv->hd; p.page = kv->page; p.kv_base = kv->kv_base;
     p.max_pos = max_pos; p.num_blocks = kv->num_blocks; p.oob_count = oob_count; p.q_len = q_len; p.row_seq = row_seq;
     p.scale_base = kv->scale_base; p.kv_int8 = kv->kv_dtype == MI355_KV_INT8; p.q_out = (f16*)q_out;
+    p.slots = to.slots; p.nseq = to.nseq; p.key_pos = to.key_pos; p.weights = to.weights;
     const uintptr_t at = (uintptr_t)qkv_f16 | (uintptr_t)qkv_bias | (uintptr_t)cos_sin | (uintptr_t)q_out | (uintptr_t)kv->kv_base;
     // Few waves: a block's two trips of 16 bytes a thread take longer than one wave's single one.  28 over 4 heads of 128, us by waves / by blocks: 64 rows 3.2 / 3.9, 192 3.9 / 4.1, 265 4.5 / 4.2; 5 over 1, 512
     // rows 3.4 / 4.4, 1055 4.4 / 4.3.  Heads of 64 (one trip): 64 rows 2.9 / 2.9, 192 3.2 / 3.2.
     if (T >= 64 && (kv->hd == 64 || (long)T * nheads >= 7400) && qkv_f16 && !p.kv_int8 && at % 16 == 0 && ld % 8 == 0) {
         const dim3 grid(cdiv(T, RP_ROWS), cdiv(nh + kv->nkv, RP_HEADS) + kv->nkv);
         hipStream_t st = (hipStream_t)stream;
-        if (kv->hd == 128) { if (bf) hipLaunchKernelGGL((rope_kv_prompt_kernel<true, 128>), grid, dim3(256), 0, st, p);
-                             else    hipLaunchKernelGGL((rope_kv_prompt_kernel<false, 128>), grid, dim3(256), 0, st, p); }
-        else               { if (bf) hipLaunchKernelGGL((rope_kv_prompt_kernel<true, 64>), grid, dim3(256), 0, st, p);
-                             else    hipLaunchKernelGGL((rope_kv_prompt_kernel<false, 64>), grid, dim3(256), 0, st, p); }
+        if (kv->hd == 128) { if (bf) hipLaunchKernelGGL((rope_kv_prompt_kernel<true, 128, SLOTS>), grid, dim3(256), 0, st, p);
+                             else    hipLaunchKernelGGL((rope_kv_prompt_kernel<false, 128, SLOTS>), grid, dim3(256), 0, st, p); }
+        else               { if (bf) hipLaunchKernelGGL((rope_kv_prompt_kernel<true, 64, SLOTS>), grid, dim3(256), 0, st, p);
+                             else    hipLaunchKernelGGL((rope_kv_prompt_kernel<false, 64, SLOTS>), grid, dim3(256), 0, st, p); }
         MI355_CHECK_LAUNCH("rope_kv_prompt_kernel");
         return MI355_OK;
     }
     if (bf)
-        hipLaunchKernelGGL(rope_kv_write_kernel<true>, dim3(T, cdiv(nheads, 4)), dim3(256), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((rope_kv_write_kernel<true, SLOTS>), dim3(T, cdiv(nheads, 4)), dim3(256), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(rope_kv_write_kernel<false>, dim3(T, cdiv(nheads, 4)), dim3(256), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((rope_kv_write_kernel<false, SLOTS>), dim3(T, cdiv(nheads, 4)), dim3(256), 0, (hipStream_t)stream, p);
     MI355_CHECK_LAUNCH("rope_kv_write_kernel");
     return MI355_OK;
+}
+} // namespace
+
+// row_seq non-null (device, [T]): the sequence of every row; q_len is 1 then
+extern "C" int mi355_rope_kv_write_rows_ragged(const void* qkv_f16, const float* partials, int32_t nsplit, int32_t ld,
+                                               const void* qkv_bias, const float* cos_sin, int32_t rope_dim, int32_t max_pos,
+                                               const int32_t* positions, const int32_t* row_seq, const int32_t* block_table, int32_t max_blocks_per_seq,
+                                               int32_t T, int32_t q_len, int32_t nh, const mi355_kv_layer_t* kv, void* q_out,
+                                               int32_t* oob_count, mi355_stream_t stream) {
+    return launch_rope<false>(qkv_f16, partials, nsplit, ld, qkv_bias, cos_sin, rope_dim, max_pos, positions, row_seq, block_table, max_blocks_per_seq, T, q_len, nh, kv, q_out,
+                              oob_count, RopeSlots{}, stream);
+}
+
+extern "C" int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias, const float* cos_sin, int32_t max_pos, const int32_t* positions, const int32_t* slots,
+                                         const int32_t* row_seq, const int32_t* block_table, int32_t max_blocks_per_seq, int32_t nseq, int32_t T, int32_t q_len, int32_t nh,
+                                         const mi355_kv_layer_t* kv, void* q_out, int32_t* key_pos, float* weights, int32_t* oob_count, mi355_stream_t stream) {
+    MI355_CHECK_ARG(qkv && slots && kv, "rope_kv_write_slots: null pointer");
+    MI355_CHECK_ARG(nseq > 0 && q_len > 0 && (row_seq ? q_len == 1 : (long)nseq * q_len == T), "rope_kv_write_slots: %d rows, %d sequences, q_len=%d (1 where the rows' sequences are given)", T, nseq, q_len);
+    MI355_CHECK_ARG((long)max_blocks_per_seq * kv->page < (1l << 31), "rope_kv_write_slots: %d blocks of %d tokens a sequence", max_blocks_per_seq, kv->page);
+    return launch_rope<true>(qkv, nullptr, 0, ld, qkv_bias, cos_sin, kv->hd, cos_sin ? max_pos : 0x7fffffff, positions, row_seq, block_table, max_blocks_per_seq, T, q_len, nh, kv,
+                             q_out, oob_count, RopeSlots{slots, nseq, key_pos, weights}, stream);
 }

@@ -30,6 +30,11 @@ def alloc_layer_cache(num_blocks: int, nkv: int, page: int, hd: int, int8: bool,
     return kv, sc
 
 
+def alloc_planes(num_blocks: int, nkv: int, page: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The planes of a cache that evicts, (attention weights fp32, positions int32), [num_blocks, nkv, page] each as the scale plane of one of K and V."""
+    return (torch.zeros(num_blocks, nkv, page, dtype=torch.float32, device=device), torch.zeros(num_blocks, nkv, page, dtype=torch.int32, device=device))
+
+
 def _flip(x: torch.Tensor) -> torch.Tensor:
     """signed code <-> stored byte (top bit flipped)."""
     return torch.bitwise_xor(x, torch.tensor(-128, dtype=torch.int8, device=x.device))
