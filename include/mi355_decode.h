@@ -407,7 +407,7 @@ int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias,
  *   max_seq_len): causal rows have end = slot + 1, a window begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = the document's
  *   first slot.  A row that sees nothing gets zeros and a log-sum-exp of -inf.  Block ids are clamped into the pool; what slots that no row of a sequence sees hold, NaN
  *   included, does not matter.
- *   q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows behind the last are left alone), or, row_start null,
+ *   Pages of whole 16 tokens.  q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows behind the last are left alone), or, row_start null,
  *   b q_len .. and rows = B q_len.  out [rows][nh hd]; lse [rows][nh] (fp32, natural logarithm) or null.  Any number of heads per kv head.
  *   weights (plane, or null): for every slot below the largest end of its sequence's rows that see something, weights <- decay weights + the sum over the sequence's rows and the heads of the
  *   kv head of exp(s - lse) (decay 1: accumulated since the start; 0: the last call's alone, whatever was there; between: fading).

@@ -8,7 +8,7 @@ from tests.scored_util import attend, bounds, gather_plane, make_cache
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-HEADS = [(28, 4, 128, 16), (14, 2, 64, 64), (8, 8, 128, 24), (8, 2, 64, 16), (6, 2, 64, 32), (71, 1, 64, 16), (40, 2, 128, 40), (16, 1, 128, 16)]
+HEADS = [(28, 4, 128, 16), (14, 2, 64, 64), (8, 8, 128, 48), (8, 2, 64, 16), (6, 2, 64, 32), (71, 1, 64, 16), (40, 2, 128, 80), (16, 1, 128, 16)]
 
 
 def run_case(nh, nkv, hd, page, dtype, int8, ctx, rows, mask, cap, bias, track, *, decay=1.0, lse=True, seed=0, qscale=2.0):
