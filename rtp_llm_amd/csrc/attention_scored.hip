@@ -422,7 +422,6 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
 
 // What the runs left: a wave per (pair, column) merges its parts (nothing to do where there is one; zeros where there is none), and, behind those blocks, a thread per slot adds the
 // probabilities of all columns to the slot's weight.
-constexpr int JOIN_COLS = 32;
 template <int HD, bool BF>
 __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, int join_blocks, int chunks) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -473,7 +472,7 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
         return;
     }
     // ---- weights
-    __shared__ float s_m[JOIN_COLS], s_i[JOIN_COLS];
+    __shared__ float s_m[32], s_i[32];
     const int id = blockIdx.x - join_blocks, pair = id / chunks, chunk = id - pair * chunks;
     const int4 mt = p.meta[pair];
     if (chunk * 1024 >= mt.w) return;
@@ -531,115 +530,544 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
         for (int e = 0; t + e < mt.w; ++e) to[e] = scored_decayed(p, to[e], sum[e]);
 }
 
-// ================================================================================================ simple forms: a wave per (row, head)
-template <int HD, bool BF, bool INT8>
-__global__ __launch_bounds__(256) void scored_rows_kernel(const ScoredParams p) {
-    __shared__ float qs[4][HD], ps[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.y, col = blockIdx.x * 4 + wave;
+// ================================================================================================ many rows
+// A wave owns 32 (row, head) pairs of a sequence's key/value head as the columns of v_mfma_f32_32x32x16, a block NW times as many: pairs lie row by row, the heads of a row side by side, so
+// any number of heads per kv head fills the tiles, and a tile spans few rows (its keys end soon behind its rows).  S^T = K q^T takes 32 keys as rows in the order
+// 16 (i / 2) + 8 half + 4 (i & 1) + r for row 8 i + 4 half + r: what a lane then holds of its column are two runs of eight keys, the second product's operand as it stands.
+// Keys and values come 64 at a time through LDS for all waves: by DMA, two steps ahead of the products with one barrier a step (three stages), or, 8 bits, through registers, which widen them
+// once for all waves.  A key's 16-byte pieces are swizzled by its low bits, a channel's 16 tokens lie side by side: no bank conflicts in either product's reads.
+struct ChunkParams : ScoredParams {
+    float*  tmp_out;       // [parts][nkv][rows G][hd] (parts > 1)
+    float4* tmp_ml;        // [parts][nkv][rows G]: maximum, sum, the reference of biases
+    float4* ml_all;        // [nkv][rows G]: maximum, 1 / sum, the reference, of every column (with weights)
+    int     tiles, parts;  // column tiles of the longest sequence, parts of the keys
+    uint32_t g_magic;      // 2^32 / G + 1
+};
+// the same for columns of queries, which lanes read one after the other
+template <int CK> __device__ __forceinline__ int swizzle_q(int c) { return c & (CK - 1); }
+// a key's swizzle: distinct over the keys that eight (rows of 128 bytes) or sixteen (256) neighbouring lanes read
+template <int CK> __device__ __forceinline__ int swizzle_of(int t) { return CK == 16 ? t & 15 : (t & 3) | (t >> 3 & 1) << 2; }
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <bool BF> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else              return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+enum { FORM_PLAIN, FORM_CAP, FORM_BIAS };           // FORM_BIAS: capped or not
+
+template <int HD, bool INT8, int NW> struct Stage {
+    static constexpr int KEYS = 64, KB = KEYS * HD * 2, BYTES = 2 * KB + (INT8 ? 2 * KEYS * 4 : 0), N = INT8 ? 2 : 3, LDS = N * BYTES + 64;
+};
+
+template <int HD, bool INT8, bool BF, int FORM, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkParams p) {
+    using ST = Stage<HD, INT8, NW>;
+    constexpr int KS = HD / 16, NDB = HD / 32, KB = ST::KB, ROW = HD * 2, CK = ROW / 16;
+    constexpr float VS = INT8 && !BF ? 64.f : 1.f, DEFER = INT8 && !BF ? 0.f : 6.f;      // as in scored_decode_kernel
+    extern __shared__ __attribute__((aligned(16))) char ch_sm[];
+    int* lim = reinterpret_cast<int*>(ch_sm + ST::N * ST::BYTES);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    // late tiles, which see most, first; a sequence's and head's blocks are B nkv parts apart, on one XCD where 8 divides that
+    int id = blockIdx.x;
+    const int part = id % p.parts; id /= p.parts;
+    const int kh = id % p.nkv; id /= p.nkv;
+    const int b = id % p.B, tile = p.tiles - 1 - id / p.B;
     int base, len;
     scored_rows_of(p, b, base, len);
-    if (col >= len * p.nh) return;
-    const int row = base + col / p.nh, h = col % p.nh, kh = h / p.G;
+    const int ncol = len * p.G, c0 = tile * 32 * NW + wave * 32;
+    if (tile * 32 * NW >= ncol) return;
+    const bool ok = c0 + col < ncol;
+    const int cc = min(c0 + col, ncol - 1), rl = cc / p.G, row = base + rl, h = kh * p.G + cc - rl * p.G;
     int lo, hi;
     scored_interval(p, row, lo, hi);
+    if (!ok) lo = hi = 0;
+    const bool seen = hi > lo;
+    if (tid == 0) { lim[0] = 0x7fffffff; lim[1] = 0; }
+    __syncthreads();
+    // [wlo, whi): what some column of the wave sees; [ilo, ihi): what all do (columns that see nothing do not count)
+    int wlo = seen ? lo : 0x7fffffff, whi = hi, ilo = lo, ihi = seen ? hi : 0x7fffffff;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        wlo = min(wlo, __shfl_xor(wlo, o)); whi = max(whi, __shfl_xor(whi, o));
+        ilo = max(ilo, __shfl_xor(ilo, o)); ihi = min(ihi, __shfl_xor(ihi, o));
+    }
+    if (lane == 0) { atomicMin(&lim[0], wlo); atomicMax(&lim[1], whi); }
+    __syncthreads();
+    wlo = __builtin_amdgcn_readfirstlane(wlo); whi = __builtin_amdgcn_readfirstlane(whi); ilo = __builtin_amdgcn_readfirstlane(ilo); ihi = __builtin_amdgcn_readfirstlane(ihi);
+    const int seen0 = __builtin_amdgcn_readfirstlane(lim[0]), khi = __builtin_amdgcn_readfirstlane(lim[1]), klo = khi > 0 ? seen0 & ~63 : 0;
+    const int all = (khi - klo + 63) / 64, s0 = (int)((long)all * part / p.parts), s1 = (int)((long)all * (part + 1) / p.parts);     // this part's steps
+
+    u32x4 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + (size_t)row * p.ldq + h * HD + s * 16 + half * 8);
+        if (!ok) qf[s] = u32x4{0u, 0u, 0u, 0u};
+    }
+    const int ref = FORM == FORM_BIAS && khi > 0 ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, khi)) : 0;
+    const float slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
+    f32x16 o[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = NEG_BIG, l = 0.f;
+
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
-    for (int d = lane; d < HD; d += 64) qs[wave][d] = act_from_bits<BF>(reinterpret_cast<const uint16_t*>(p.q)[(size_t)row * p.ldq + h * HD + d]);
-    __builtin_amdgcn_wave_barrier();
-    const float slope = p.slopes ? p.slopes[h] : 0.f;
-    const int qp = p.slopes ? p.positions[row] : 0;
-    float m = NEG_BIG, l = 0.f, o[HD / 64];
-#pragma unroll
-    for (int c = 0; c < HD / 64; ++c) o[c] = 0.f;
-    for (int t0 = lo; t0 < hi; t0 += 64) {
-        const int t = t0 + lane;
-        const bool ok = t < hi;
-        const int tc = ok ? t : hi - 1;
-        const int blk = scored_block(p, bt, tc), ti = tc % p.page;
-        const size_t hk = ((size_t)blk * 2) * p.nkv + kh, hv = hk + p.nkv;
-        float s = 0.f;
-        for (int d = 0; d < HD; ++d) {
-            const size_t at = (hk * p.page + ti) * HD + d;
-            const float k = INT8 ? (float)((int)reinterpret_cast<const uint8_t*>(p.kv_base)[at] - 128) : act_from_bits<BF>(reinterpret_cast<const uint16_t*>(p.kv_base)[at]);
-            s = __builtin_fmaf(qs[wave][d], k, s);
+    const int last16 = khi > 0 ? (khi - 1) & ~15 : 0;
+    auto page_of = [&](int t) { return (int)__builtin_amdgcn_readfirstlane((int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)); };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ch_sm;
+    int idv = 0;                                    // block ids of 16 steps' units of 16 keys, a lane each
+    auto ids_for = [&](int st) {
+        if (((st - s0) & 15) == 0) {
+            const int t = min(klo + st * 64 + lane * 16, last16);
+            idv = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
         }
-        if (INT8) s *= p.scale_base[hk * p.page + ti];
-        s *= p.scale1;
-        if (p.capped) s = p.cap_log2 * (fabsf(s) <= kTanhNear ? tanh_near(s) : tanh_far(s));
-        if (p.slopes) {
-            const int kp = p.key_pos ? p.key_pos[((size_t)blk * p.nkv + kh) * p.page + ti] : tc;
-            s = __builtin_fmaf(slope * kLog2e, (float)(kp - qp), s);
+    };
+    // base of a unit's keys and values; a unit past the last seen slot is that one's again (masked)
+    const uint32_t head_elems = (uint32_t)(p.page * HD);
+    auto unit_at = [&](int st, int u, int& ti, uint32_t& hk) {
+        const int t = min(klo + st * 64 + u * 16, last16);
+        ti = t - page_of(t) * p.page;
+        hk = (uint32_t)min(max(__builtin_amdgcn_readlane(idv, ((st - s0) & 15) * 4 + u), 0), p.num_blocks - 1) * (uint32_t)(2 * p.nkv) + (uint32_t)kh;
+    };
+    // ---- 16 bits: 1 KB loads, KL of keys (1024 / ROW keys each) and as many of values (32 channels of a unit each) a stage
+    constexpr int KL = KB / 1024, JK = KL / NW, KU = KL / 4;                          // loads of keys a stage, a wave, a unit
+    const int krow = (wave % KU) * (1024 / ROW) + lane / CK;
+    const uint32_t koff = (uint32_t)(krow * ROW + (((lane % CK) ^ swizzle_of<CK>(krow)) << 4)), voff = (uint32_t)((lane >> 1) * p.page + (lane & 1) * 8) * 2u;
+    auto issue = [&](int st, int buf) {
+        ids_for(st);
+#pragma unroll
+        for (int j = 0; j < JK; ++j) {
+            const int d = j * NW + wave;
+            int ti; uint32_t hk;
+            unit_at(st, d / KU, ti, hk);
+            const uint16_t* kb = (const uint16_t*)p.kv_base + (uint64_t)hk * head_elems;
+            const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buf * ST::BYTES + d * 1024);
+            uint32_t ko = koff;
+            if constexpr (KU > NW) {                // the rows differ from load to load
+                const int r = (d % KU) * (1024 / ROW) + lane / CK;
+                ko = (uint32_t)(r * ROW + (((lane % CK) ^ swizzle_of<CK>(r)) << 4));
+            }
+            dma16(to, ko, kb + (uint32_t)(ti * HD));
+            dma16(to + KB, voff, kb + (uint64_t)(uint32_t)p.nkv * head_elems + (uint32_t)ti + (uint32_t)(d % KU * 32) * (uint32_t)p.page);
         }
-        s = ok ? s : NEG_BIG;
-        const float mn = fmaxf(m, wave_max(s)), alpha = __builtin_amdgcn_exp2f(m - mn);
-        const float pe = ok ? __builtin_amdgcn_exp2f(s - mn) : 0.f;
-        l = l * alpha + wave_sum(pe);
-        m = mn;
-        ps[wave][lane] = INT8 ? (ok ? pe * p.scale_base[hv * p.page + ti] : 0.f) : pe;
-        __builtin_amdgcn_wave_barrier();
+    };
+    // ---- 8 bits: 16-byte pieces through registers, a thread takes the same piece numbers of every stage
+    constexpr int PIECES = 64 * HD / 16, JP = INT8 ? (PIECES + 64 * NW - 1) / (64 * NW) : 1;
+    u32x4 rk[JP], rv[JP];
+    float rs = 0.f;
+    auto fetch8 = [&](int st) {
+        ids_for(st);
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) o[c] *= alpha;
-        const int n = min(64, hi - t0);
-        for (int j = 0; j < n; ++j) {
-            const int bj = __shfl(blk, j), tj = (t0 + j) % p.page;
-            const size_t vb = ((size_t)bj * 2 + 1) * p.nkv + kh;
+        for (int j = 0; j < JP; ++j) {
+            const int i = j * 64 * NW + tid, u = __builtin_amdgcn_readfirstlane(i / HD);          // HD pieces a unit: whole waves (HD 64, 128)
+            int ti; uint32_t hk;
+            unit_at(st, min(u, 3), ti, hk);
+            const char* kb = (const char*)p.kv_base + (uint64_t)hk * head_elems;
+            const int q = i % HD;
+            rk[j] = *reinterpret_cast<const u32x4*>(kb + ti * HD + q * 16);
+            rv[j] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)(uint32_t)p.nkv * head_elems + q * p.page + ti);
+        }
+        if (tid < 128) {                            // scales: 64 of keys, 64 of values
+            const int t = min(klo + st * 64 + (tid & 63 & ~15), last16), blk = __shfl(idv, ((st - s0) & 15) * 4 + ((tid & 63) >> 4));
+            const size_t hk = (size_t)min(max(blk, 0), p.num_blocks - 1) * 2 * p.nkv + kh + (tid >= 64 ? p.nkv : 0);
+            rs = p.scale_base[hk * p.page + t % p.page + (tid & 15)];
+        }
+    };
+    auto store8 = [&](int buf) {
+        char* st = ch_sm + buf * ST::BYTES;
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c) {
-                const size_t at = (vb * HD + lane + 64 * c) * p.page + tj;
-                const float v = INT8 ? (float)((int)reinterpret_cast<const uint8_t*>(p.kv_base)[at] - 128) : act_from_bits<BF>(reinterpret_cast<const uint16_t*>(p.kv_base)[at]);
-                o[c] = __builtin_fmaf(ps[wave][j], v, o[c]);
+        for (int j = 0; j < JP; ++j) {
+            const int i = j * 64 * NW + tid;
+            if (PIECES % (64 * NW) && i >= PIECES) break;
+            const int t = i / (HD / 16), c = (i % (HD / 16)) * 2, f = swizzle_of<CK>(t & 15);
+            *reinterpret_cast<u32x4*>(st + t * ROW + ((c ^ f) << 4)) = widen_codes<BF>(rk[j][0], rk[j][1]);
+            *reinterpret_cast<u32x4*>(st + t * ROW + (((c + 1) ^ f) << 4)) = widen_codes<BF>(rk[j][2], rk[j][3]);
+            *reinterpret_cast<u32x4*>(st + KB + i * 32) = widen_codes<BF>(rv[j][0], rv[j][1]);
+            *reinterpret_cast<u32x4*>(st + KB + i * 32 + 16) = widen_codes<BF>(rv[j][2], rv[j][3]);
+        }
+        if (tid < 128) reinterpret_cast<float*>(st + 2 * KB)[tid] = rs;
+    };
+
+    // where the lane's fragments lie: its key in a group of 32, that key's pieces
+    const int kt = 16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3), kf = swizzle_of<CK>(kt & 15);
+    auto compute = [&](const char* st, int t0, auto masked_c) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        float sv[2][16];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            f32x16 s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                s = mfma32<BF>(*reinterpret_cast<const u32x4*>(st + (g * 32 + kt) * ROW + (((ks * 2 + half) ^ kf) << 4)), qf[ks], s);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sv[g][i] = s[i];
+        }
+        // sv[g][8 kk + e] is key t0 + 32 g + 16 kk + 8 half + e
+        if constexpr (INT8) {
+            const f32x4* sc = reinterpret_cast<const f32x4*>(st + 2 * KB) + half * 2;
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sv[g][i] *= sc[g * 8 + (i >> 3) * 4 + (i >> 2 & 1)][i & 3];
+        }
+        float mul = p.scale1;                       // scores are sv times mul from here on
+        if constexpr (FORM != FORM_PLAIN) {
+            if (FORM == FORM_CAP || p.capped) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[g][i] *= p.scale1;
+                    tanh_all(sv[g]);
+                }
+                mul = p.cap_log2;
             }
         }
-        __builtin_amdgcn_wave_barrier();
-    }
-    const float inv = scored_inv(l, hi > lo);
+        if constexpr (FORM == FORM_BIAS) {
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) reinterpret_cast<uint16_t*>(p.out)[((size_t)row * p.nh + h) * HD + lane + 64 * c] = act_to_bits<BF>(o[c] * inv);
-    if (lane == 0 && p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, hi > lo, 0.f);
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int t = t0 + g * 32 + (k >> 1) * 16 + half * 8 + (k & 1) * 4;
+                    i32x4 kp = {t - ref, t + 1 - ref, t + 2 - ref, t + 3 - ref};
+                    if (p.key_pos) {                // the planes' rows of four tokens lie inside a page
+                        const int tc = min(t, last16 + 12), blk = scored_block(p, bt, tc);
+                        kp = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)blk * p.nkv + kh) * p.page + tc % p.page);
+                        kp -= ref;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sv[g][k * 4 + e] = __builtin_fmaf(slope2, (float)kp[e], sv[g][k * 4 + e] * mul);
+                }
+            mul = 1.f;
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (MASKED) {
+                    const int t = t0 + g * 32 + (i >> 3) * 16 + half * 8 + (i & 7);
+                    sv[g][i] = t >= lo && t < hi ? sv[g][i] : -__builtin_inff();
+                }
+                mx = fmaxf(mx, sv[g][i]);
+            }
+        mx = fmaxf(xor32_max(mx) * mul, NEG_BIG);
+        if (__builtin_amdgcn_ballot_w64(mx > m + DEFER)) {
+            const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) o[d] *= alpha;
+            m = mn;
+        }
+        float psum = 0.f;
+        u32x4 pf[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float pe[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                pe[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[k >> 1][(k & 1) * 8 + e], mul, -m));
+                psum += pe[e];
+                if constexpr (INT8) {
+                    const float vs = (reinterpret_cast<const float*>(st + 2 * KB) + 64)[k * 16 + half * 8 + e] * VS;
+                    const int t = t0 + k * 16 + half * 8 + e;
+                    pe[e] = !MASKED || (t >= lo && t < hi) ? pe[e] * vs : 0.f;
+                }
+            }
+            pf[k] = act_pack8<BF>(pe);
+        }
+        l += psum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) {
+                u32x4 a = *reinterpret_cast<const u32x4*>(st + KB + (k * HD + d * 32 + col) * 32 + half * 16);
+                if (MASKED && !INT8 && (t0 + 64 > khi || t0 < seen0)) {     // slots that no row here sees may hold anything, NaN too: their weights are zero, their values are made so
+                    const int t = t0 + k * 16 + half * 8;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (t + e >= khi || t + e < seen0) a[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+                }
+                o[d] = mfma32<BF>(a, pf[k], o[d]);
+            }
+    };
+    auto step = [&](const char* st, int t0) {
+        if (t0 >= whi || t0 + 64 <= wlo) return;
+        if (t0 >= ilo && t0 + 64 <= ihi) compute(st, t0, std::false_type{});
+        else compute(st, t0, std::true_type{});
+    };
+    wait_vm<0>();                                   // the queries are here: no wait for them inside the loop
+    if constexpr (!INT8) {
+        constexpr int NS = ST::N;
+        for (int i = 0; i < min(NS - 1, s1 - s0); ++i) issue(s0 + i, i);
+        int buf = 0;
+        for (int st = s0; st < s1; ++st) {
+            if (st + 1 < s1) wait_vm<2 * JK * (NS - 2)>(); else wait_vm<0>();        // this step's loads of this wave (the next step's may be left)
+            __builtin_amdgcn_s_barrier();           // everyone's; and everyone is done with the stage before
+            asm volatile("" ::: "memory");
+            if (st + NS - 1 < s1) issue(st + NS - 1, buf == 0 ? NS - 1 : buf - 1);
+            step(ch_sm + buf * ST::BYTES, klo + st * 64);
+            buf = buf == NS - 1 ? 0 : buf + 1;
+        }
+    } else if (s0 < s1) {
+        fetch8(s0);
+        store8(0);
+        if (s0 + 1 < s1) fetch8(s0 + 1);
+        int buf = 0;
+        for (int st = s0; st < s1; ++st) {
+            __syncthreads();                        // this stage is whole, and everyone is done with the other one
+            if (st + 1 < s1) { store8(buf ^ 1); if (st + 2 < s1) fetch8(st + 2); }
+            step(ch_sm + buf * ST::BYTES, klo + st * 64);
+            buf ^= 1;
+        }
+    }
+    l = xor32_sum(l);
+    if (!ok) return;
+    const size_t at = (size_t)kh * p.rows * p.G + (size_t)base * p.G + cc;           // the column among all of its kv head
+    if (p.parts > 1) {
+        const size_t slot = (size_t)part * p.nkv * p.rows * p.G + at;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 v = {o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+                if constexpr (VS != 1.f) v *= 1.f / VS;
+                *reinterpret_cast<f32x4*>(p.tmp_out + slot * HD + d * 32 + i * 8 + half * 4) = v;
+            }
+        if (half == 0) p.tmp_ml[slot] = make_float4(m, l, __builtin_bit_cast(float, ref), 0.f);
+        return;
+    }
+    const float inv = scored_inv(l, seen) * (1.f / VS);
+    uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + ((size_t)row * p.nh + h) * HD + half * 4;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u32x2 v = {0u, 0u};
+            if (seen) { v[0] = act_pack<BF>(o[d][i * 4] * inv, o[d][i * 4 + 1] * inv); v[1] = act_pack<BF>(o[d][i * 4 + 2] * inv, o[d][i * 4 + 3] * inv); }
+            *reinterpret_cast<u32x2*>(out + d * 32 + i * 8) = v;
+        }
+    if (half == 0) {
+        if (p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, seen, seen ? scored_shift(p, row, h, ref) : 0.f);
+        if (p.ml_all) p.ml_all[at] = make_float4(m, scored_inv(l, seen), __builtin_bit_cast(float, ref), 0.f);
+    }
 }
 
-// A thread per (slot, kv head): the probabilities of all rows and heads that see it.
-template <int HD, bool BF, bool INT8>
-__global__ __launch_bounds__(256) void scored_weights_kernel(const ScoredParams p) {
-    const int b = blockIdx.z, kh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
+// Parts of the keys into results: a wave per column.
+template <int HD, bool BF>
+__global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) {
+    const int lane = threadIdx.x & 63;
+    const size_t cols = (size_t)p.rows * p.G, at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= cols * p.nkv) return;
+    const int kh = (int)(at / cols), c = (int)(at - kh * cols), row = c / p.G, h = kh * p.G + c - row * p.G;
+    constexpr int CPL = HD / 64;
+    float m = NEG_BIG, l = 0.f, acc[CPL];
+    int ref = 0;
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) acc[k] = 0.f;
+    int b = row / p.q_len;
+    if (p.row_start) {                              // the row's sequence; a row behind the last has no parts
+        int lo = 0, hi = p.B;
+        while (lo < hi) { const int mid = (lo + hi) >> 1; if (p.row_start[mid + 1] > row) hi = mid; else lo = mid + 1; }
+        b = lo;
+        if (b >= p.B) return;
+        int base, len;
+        scored_rows_of(p, b, base, len);
+        if (row < base || row >= base + len) return;
+    }
+    const int np = p.parts;
+    for (int i = 0; i < np; ++i) m = fmaxf(m, p.tmp_ml[i * cols * p.nkv + at].x);
+    for (int i = 0; i < np; ++i) {
+        const size_t slot = i * cols * p.nkv + at;
+        const float4 ml = p.tmp_ml[slot];
+        ref = __builtin_bit_cast(int, ml.z);
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l += ml.y * f;
+#pragma unroll
+        for (int k = 0; k < CPL; ++k) acc[k] += p.tmp_out[slot * HD + lane * CPL + k] * f;
+    }
+    int a, e;
+    scored_interval(p, row, a, e);
+    const bool seen = e > a;
+    const float inv = scored_inv(l, seen);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((size_t)row * p.nh + h) * HD + lane * CPL;
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) dst[k] = act_to_bits<BF>(seen ? acc[k] * inv : 0.f);
+    if (lane == 0) {
+        if (p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, seen, seen ? scored_shift(p, row, h, ref) : 0.f);
+        if (p.ml_all) p.ml_all[at] = make_float4(m, inv, __builtin_bit_cast(float, ref), 0.f);
+    }
+}
+
+// The weights of many rows: S^T once more, a wave's 32 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 128 keys, its 16 waves four groups of 32
+// columns of each 128 at a time; a probability is added in the lane of its column, lanes and groups meet once at the end: no atomics, the same sums every time.
+template <int HD, bool INT8, bool BF, int FORM>
+__global__ __launch_bounds__(1024) void scored_sums_kernel(const ChunkParams p, int key_tiles) {
+    constexpr int KS = HD / 16, ROW = HD * 2, CK = ROW / 16, QB = 128 * ROW, LOADS = QB / 1024, JL = LOADS / 16;
+    extern __shared__ __attribute__((aligned(16))) char su_sm[];
+    struct Col { float m, inv, slope2; int ref, lo, hi, pad0, pad1; };
+    static_assert(sizeof(Col) == 32, "");
+    Col* cols = reinterpret_cast<Col*>(su_sm + 2 * QB);              // [2][128]
+    float* meet = reinterpret_cast<float*>(su_sm);                   // [3][128], over the columns when they are done
+    int* s_reach = reinterpret_cast<int*>(su_sm + 2 * QB + 2 * 128 * sizeof(Col));
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5, cg = wave >> 2;
+    int id = blockIdx.x;
+    const int tile = id % key_tiles; id /= key_tiles;
+    const int kh = id % p.nkv, b = id / p.nkv;
     int base, len;
     scored_rows_of(p, b, base, len);
+    const int ncol = len * p.G, tw = tile * 128 + (wave & 3) * 32;    // the wave's first slot
+    if (tid == 0) *s_reach = 0;
+    __syncthreads();
     int reach = 0;
-    for (int i = 0; i < len; ++i) { int lo, hi; scored_interval(p, base + i, lo, hi); reach = max(reach, hi); }
-    if (t >= reach) return;
+    for (int i = tid; i < len; i += 1024) { int a, e; scored_interval(p, base + i, a, e); reach = max(reach, e); }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) reach = max(reach, __shfl_xor(reach, o));
+    if (lane == 0) atomicMax(s_reach, reach);
+    __syncthreads();
+    reach = __builtin_amdgcn_readfirstlane(*s_reach);
+    if (tile * 128 >= reach) return;
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
-    const int raw = bt[t / p.page];
-    if (raw < 0 || raw >= p.num_blocks) return;
-    const int ti = t % p.page;
-    const size_t hk = ((size_t)raw * 2) * p.nkv + kh, wat = ((size_t)raw * p.nkv + kh) * p.page + ti;
-    float sum = 0.f;
-    for (int i = 0; i < len; ++i) {
-        int lo, hi;
-        scored_interval(p, base + i, lo, hi);
-        if (t < lo || t >= hi) continue;
-        for (int h = kh * p.G; h < kh * p.G + p.G; ++h) {
-            float s = 0.f;
-            for (int d = 0; d < HD; ++d) {
-                const size_t at = (hk * p.page + ti) * HD + d;
-                const float k = INT8 ? (float)((int)reinterpret_cast<const uint8_t*>(p.kv_base)[at] - 128) : act_from_bits<BF>(reinterpret_cast<const uint16_t*>(p.kv_base)[at]);
-                s = __builtin_fmaf(act_from_bits<BF>(reinterpret_cast<const uint16_t*>(p.q)[(size_t)(base + i) * p.ldq + h * HD + d]), k, s);
+    u32x4 kfr[KS];
+    float ksc[INT8 ? 16 : 1];
+    i32x4 kp[FORM == FORM_BIAS ? 4 : 1];
+    {
+        const int t = min(tw + col, reach - 1), blk = scored_block(p, bt, t);
+        const size_t at = (((size_t)blk * 2) * p.nkv + kh) * p.page + t % p.page;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (INT8) {
+                const u32x2 v = *reinterpret_cast<const u32x2*>((const char*)p.kv_base + at * HD + s * 16 + half * 8);
+                kfr[s] = widen_codes<BF>(v[0], v[1]);
+            } else kfr[s] = *reinterpret_cast<const u32x4*>((const uint16_t*)p.kv_base + at * HD + s * 16 + half * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                                // the lane's results are keys 8 i + 4 half + r
+            const int tt = tw + i * 8 + half * 4, tc = min(tt, (reach - 1) & ~3), bl = scored_block(p, bt, tc);
+            if constexpr (INT8) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(p.scale_base + (((size_t)bl * 2) * p.nkv + kh) * p.page + tc % p.page);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ksc[i * 4 + e] = v[e];
             }
-            if (INT8) s *= p.scale_base[hk * p.page + ti];
-            s *= p.scale1;
-            if (p.capped) s = p.cap_log2 * (fabsf(s) <= kTanhNear ? tanh_near(s) : tanh_far(s));
-            if (p.slopes) s = __builtin_fmaf(p.slopes[h] * kLog2e, (float)((p.key_pos ? p.key_pos[wat] : t) - p.positions[base + i]), s);
-            sum += __builtin_amdgcn_exp2f(s - p.lse[(size_t)(base + i) * p.nh + h] * kLog2e);
+            if constexpr (FORM == FORM_BIAS) {
+                kp[i] = i32x4{tt, tt + 1, tt + 2, tt + 3};
+                if (p.key_pos) kp[i] = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)bl * p.nkv + kh) * p.page + tc % p.page);
+            }
         }
     }
-    p.weights[wat] = scored_decayed(p, p.weights[wat], sum);
+    float acc[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)su_sm;
+    const int steps = (ncol + 127) / 128;
+    auto place = [&](int c, int& row, int& h) {
+        c = min(c, ncol - 1);
+        const int r = p.G == 1 ? c : (int)(((unsigned long long)(unsigned)c * p.g_magic) >> 32);
+        row = base + r; h = kh * p.G + c - r * p.G;
+    };
+    auto issue = [&](int st, int buf) {
+#pragma unroll
+        for (int j = 0; j < JL; ++j) {
+            const int d = j * 16 + wave, cl = d * (1024 / ROW) + lane / CK;
+            int row, h;
+            place(st * 128 + cl, row, h);
+            dma16(__builtin_amdgcn_readfirstlane(lds0 + buf * QB + d * 1024), (const uint16_t*)p.q + (size_t)row * p.ldq + h * HD + ((lane % CK) ^ swizzle_q<CK>(cl)) * 8);
+        }
+    };
+    Col mine;
+    auto fetch = [&](int st) {
+        if (tid >= 128) return;
+        const int c = st * 128 + tid;
+        int row, h;
+        place(c, row, h);
+        const float4 ml = p.ml_all[(size_t)kh * p.rows * p.G + (size_t)base * p.G + min(c, ncol - 1)];
+        mine.m = ml.x; mine.inv = ml.y; mine.ref = __builtin_bit_cast(int, ml.z);
+        mine.slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
+        scored_interval(p, row, mine.lo, mine.hi);
+        if (c >= ncol) mine.lo = mine.hi = 0;
+    };
+    fetch(0);
+    issue(0, 0);
+    if (tid < 128) cols[tid] = mine;
+    wait_vm<0>();
+    for (int st = 0; st < steps; ++st) {
+        const int buf = st & 1;
+        __syncthreads();
+        if (st + 1 < steps) { issue(st + 1, buf ^ 1); fetch(st + 1); }
+        const Col c = cols[buf * 128 + cg * 32 + col];
+        if (__builtin_amdgcn_ballot_w64(c.lo < tw + 32 && c.hi > tw)) {
+            const bool masked = __builtin_amdgcn_ballot_w64(c.lo > tw || c.hi < tw + 32) != 0;
+            f32x16 s;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+            const int cl = cg * 32 + col, f = swizzle_q<CK>(cl);
+            const char* q = su_sm + buf * QB + cl * ROW;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s = mfma32<BF>(kfr[ks], *reinterpret_cast<const u32x4*>(q + (((ks * 2 + half) ^ f) << 4)), s);
+            float sv[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sv[i] = INT8 ? s[i] * ksc[INT8 ? i : 0] : s[i];
+            float mul = p.scale1;
+            if constexpr (FORM != FORM_PLAIN) {
+                if (FORM == FORM_CAP || p.capped) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[i] *= p.scale1;
+                    tanh_all(sv);
+                    mul = p.cap_log2;
+                }
+            }
+            if constexpr (FORM == FORM_BIAS) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sv[i] = __builtin_fmaf(c.slope2, (float)(kp[i >> 2][i & 3] - c.ref), sv[i] * mul);
+                mul = 1.f;
+            }
+            if (!masked) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], mul, -c.m)), c.inv, acc[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int t = tw + (i >> 2) * 8 + half * 4 + (i & 3);
+                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], mul, -c.m)) * c.inv;
+                    acc[i] += t >= c.lo && t < c.hi ? pe : 0.f;
+                }
+            }
+        }
+        if (st + 1 < steps) {
+            if (tid < 128) cols[(buf ^ 1) * 128 + tid] = mine;
+            wait_vm<0>();
+        }
+    }
+    float sum = 0.f;                                                 // lane `col` < 16 ends up with result `col`
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float v = acc[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) v += __shfl_xor(v, o);
+        if (col == i) sum = v;
+    }
+    __syncthreads();
+    const int key = (wave & 3) * 32 + (col >> 2) * 8 + half * 4 + (col & 3);
+    if (cg > 0 && col < 16) meet[(cg - 1) * 128 + key] = sum;
+    __syncthreads();
+    if (cg > 0 || col >= 16) return;
+    sum += meet[key]; sum += meet[128 + key]; sum += meet[256 + key];
+    const int t = tile * 128 + key;
+    if (t >= reach) return;
+    const int blk = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
+    if (blk < 0 || blk >= p.num_blocks) return;
+    float* to = p.weights + ((size_t)blk * p.nkv + kh) * p.page + t % p.page;
+    *to = scored_decayed(p, *to, sum);
 }
 
 // ================================================================================================ plans
-// How a call runs: sizes of its workspace's regions, each on 256 bytes.
+// How a call runs, and its workspace's regions, each on 256 bytes.
 struct Plan {
     bool   few;                // the few-row kernel: at most 32 (row, head) pairs of a key/value head a sequence
     int    nblocks, ncol, ctx_pad, runs;
-    size_t tmp_out, tmp_ml, ml_all, spill, meta, lse, bytes;     // offsets; bytes: all
+    int    waves, tiles, parts;                                  // the many-row kernel
+    size_t tmp_out, tmp_ml, ml_all, spill, meta, bytes;          // offsets; bytes: all
 };
 constexpr int RUNS = 256;      // one block of the few-row kernel a compute unit
 Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, bool track) {
@@ -647,7 +1075,7 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
     const int G = nh / nkv;
     size_t at = 0;
     auto region = [&](size_t bytes) { const size_t r = at; at += (bytes + 255) & ~(size_t)255; return r; };
-    pl.few = (long)q_len * G <= JOIN_COLS;
+    pl.few = (long)q_len * G <= 32;
     if (pl.few) {
         const long pairs = (long)B * nkv;
         pl.runs = pairs < 4 * RUNS;                              // beyond, pairs are many enough to even out by themselves, and nothing has to be merged
@@ -656,7 +1084,15 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         pl.meta = region(pairs * sizeof(int4));
         if (pl.runs) { pl.tmp_out = region((size_t)2 * RUNS * pl.ncol * hd * 4); pl.tmp_ml = region((size_t)2 * RUNS * pl.ncol * 8); }
         if (track) { pl.ml_all = region(pairs * pl.ncol * 8); pl.spill = region(pairs * pl.ncol * pl.ctx_pad * 4); }
-    } else if (track) pl.lse = region((size_t)rows * nh * 4);
+    } else {
+        const long cols = (long)q_len * G;
+        pl.waves = cols <= 64 ? 2 : cols <= 128 ? 4 : 8;
+        pl.tiles = (int)((cols + 32 * pl.waves - 1) / (32 * pl.waves));
+        const long blocks = (long)pl.tiles * B * nkv, room = 256 * 8 / pl.waves;
+        pl.parts = (int)std::max(1l, std::min({room / std::max(1l, blocks), (max_seq + 255l) / 256, 64l}));
+        if (pl.parts > 1) { pl.tmp_out = region((size_t)pl.parts * rows * nh * hd * 4); pl.tmp_ml = region((size_t)pl.parts * rows * nh * 16); }
+        if (track) pl.ml_all = region((size_t)rows * nh * 16);
+    }
     pl.bytes = at;
     return pl;
 }
@@ -669,6 +1105,30 @@ int launch_decode(const DecodeParams& d, hipStream_t st) {
         return rc;
     };
     return d.key_pos ? run(scored_decode_kernel<HD, INT8, NT, BF, true>, Ring<HD, INT8, true>::BYTES) : run(scored_decode_kernel<HD, INT8, NT, BF, false>, Ring<HD, INT8, INT8>::BYTES);
+}
+
+template <int HD, bool INT8, bool BF, int FORM>
+int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
+    auto run = [&](auto kernel, int lds, int threads, long blocks, auto... more) -> int {
+        const int rc = raise_dynamic_lds((const void*)kernel, "paged_attn_scored");
+        if (rc == MI355_OK) hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, c, more...);
+        return rc;
+    };
+    const long blocks = (long)pl.tiles * c.B * c.nkv * pl.parts;
+    int rc = pl.waves == 2 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 2>, Stage<HD, INT8, 2>::LDS, 128, blocks)
+           : pl.waves == 4 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 4>, Stage<HD, INT8, 4>::LDS, 256, blocks)
+                           : run(scored_chunk_kernel<HD, INT8, BF, FORM, 8>, Stage<HD, INT8, 8>::LDS, 512, blocks);
+    if (rc != MI355_OK) return rc;
+    if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 3) / 4)), dim3(256), 0, st, c);
+    if (c.weights) {
+        const int key_tiles = cdiv(c.max_seq, 128);
+        rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 2 * 128 * HD * 2 + 2 * 128 * 32 + 16, 1024, (long)key_tiles * c.nkv * c.B, key_tiles);
+    }
+    return rc;
+}
+template <int HD, bool INT8, bool BF>
+int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
+    return c.slopes ? launch_chunk<HD, INT8, BF, FORM_BIAS>(c, pl, st) : c.capped ? launch_chunk<HD, INT8, BF, FORM_CAP>(c, pl, st) : launch_chunk<HD, INT8, BF, FORM_PLAIN>(c, pl, st);
 }
 
 } // namespace
@@ -714,15 +1174,19 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
         MI355_CHECK_LAUNCH("scored_join_kernel");
         return MI355_OK;
     }
-    if (weights && !lse) p.lse = (float*)(ws + pl.lse);
-    const ScoredParams& sp = p;
-    const dim3 grid(cdiv(q_len * nh, 4), B), wgrid(cdiv(max_seq_len, 256), kv->nkv, B);
-#define L_(HD_, BF_, I8_) do { hipLaunchKernelGGL((scored_rows_kernel<HD_, BF_, I8_>), grid, dim3(256), 0, st, sp); \
-                               if (weights) hipLaunchKernelGGL((scored_weights_kernel<HD_, BF_, I8_>), wgrid, dim3(256), 0, st, sp); } while (0)
-#define LB_(HD_) do { if (bf) { if (int8) L_(HD_, true, true); else L_(HD_, true, false); } else { if (int8) L_(HD_, false, true); else L_(HD_, false, false); } } while (0)
+    ChunkParams c;
+    static_cast<ScoredParams&>(c) = p;
+    c.tiles = pl.tiles; c.parts = pl.parts; c.g_magic = (uint32_t)((1ull << 32) / (unsigned)p.G + 1);
+    c.tmp_out = pl.parts > 1 ? (float*)(ws + pl.tmp_out) : nullptr; c.tmp_ml = pl.parts > 1 ? (float4*)(ws + pl.tmp_ml) : nullptr;
+    c.ml_all = weights ? (float4*)(ws + pl.ml_all) : nullptr;
+    MI355_CHECK_ARG((long)pl.tiles * B * kv->nkv * pl.parts < (1l << 31) && (long)cdiv(max_seq_len, 128) * kv->nkv * B < (1l << 31) && (long)q_len * p.G * p.G < (1l << 32),
+                    "paged_attn_scored: %d rows of %d heads in %d sequences of %d slots exceed the grid", rows, nh, B, max_seq_len);
+    int crc;
+#define LB_(HD_) do { if (bf) crc = int8 ? launch_chunk<HD_, true, true>(c, pl, st) : launch_chunk<HD_, false, true>(c, pl, st); \
+                      else    crc = int8 ? launch_chunk<HD_, true, false>(c, pl, st) : launch_chunk<HD_, false, false>(c, pl, st); } while (0)
     if (kv->hd == 128) LB_(128); else LB_(64);
 #undef LB_
-#undef L_
-    MI355_CHECK_LAUNCH("paged_attn_scored");
+    if (crc != MI355_OK) return crc;
+    MI355_CHECK_LAUNCH("scored_chunk_kernel");
     return MI355_OK;
 }

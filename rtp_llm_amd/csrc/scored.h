@@ -120,7 +120,7 @@ inline int scored_params(ScoredParams& p, const void* q, int ldq, const mi355_kv
                     kv->kv_dtype, kv->act_dtype);
     MI355_CHECK_ARG((((uintptr_t)q | (uintptr_t)kv->kv_base | (uintptr_t)out) & 15) == 0 && (((uintptr_t)kv->scale_base) & 15) == 0, "paged_attn_scored: q, cache, scales and out lie on 16 bytes");
     MI355_CHECK_ARG(sc->softcap == 0.f || (sc->softcap >= 1e-6f && sc->softcap <= 1e6f), "paged_attn_scored: softcap=%g (0: none, or 1e-6 to 1e6)", (double)sc->softcap);
-    MI355_CHECK_ARG(sc->scale > -1e6f && sc->scale < 1e6f, "paged_attn_scored: scale=%g", (double)sc->scale);
+    MI355_CHECK_ARG(sc->scale > 0.f && sc->scale < 1e6f, "paged_attn_scored: scale=%g (> 0)", (double)sc->scale);
     MI355_CHECK_ARG(!sc->slopes || sc->positions, "paged_attn_scored: slopes need the rows' positions");
     MI355_CHECK_ARG(!weights || (decay >= 0.f && decay <= 1.f), "paged_attn_scored: decay=%g (0 to 1)", (double)decay);
     p.q = q; p.ldq = ldq; p.kv_base = kv->kv_base; p.scale_base = kv->scale_base; p.block_table = block_table; p.row_start = row_start;
