@@ -37,9 +37,7 @@ struct DecodeParams : ScoredParams {
 constexpr int UNIT = 128;
 
 // The slots that a sequence's rows see, [seen, hi), and lo = seen down to 32; nothing: zeros.
-__device__ __forceinline__ void scored_span(const ScoredParams& p, int b, int& lo, int& hi, int& seen) {
-    int base, len;
-    scored_rows_of(p, b, base, len);
+__device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int len, int& lo, int& hi, int& seen) {
     seen = 0x7fffffff; hi = 0;
     for (int i = 0; i < len; ++i) {
         int a, e;
@@ -105,34 +103,43 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
     // where the lane's fragments lie in a stage
     const int ktok = (j & 3) + 8 * (j >> 2), kf = ((j & 3) | (j >> 2) << 2) & (CK - 1);
 
-    // ---- this block's run of units
-    int b, kh, lo, hi, seen0, units, u, u1;                // the pair at hand, its span, the run's next unit inside it, the run's end (counted from the pair's first unit)
+    // ---- this block's run of units.  Lane i looks at sequence i of each 64; up to 64 sequences its answers are all that the block needs of them.
+    int b, kh, lo, hi, seen0, base, len, units, u, u1;  // the pair at hand, its span and rows, the run's next unit inside it, the run's end (counted from the pair's first unit)
+    int my_lo = 0, my_hi = 0, my_seen = 0, my_base = 0, my_len = 0;
+    auto look = [&](int b0) {
+        my_lo = my_hi = my_seen = my_base = my_len = 0;
+        if (b0 + lane < p.B) { scored_rows_of(p, b0 + lane, my_base, my_len); scored_span(p, my_base, my_len, my_lo, my_hi, my_seen); }
+    };
+    auto take = [&](int who) {
+        if (p.B > 64) { look(who & ~63); who &= 63; }
+        lo = __builtin_amdgcn_readlane(my_lo, who); hi = __builtin_amdgcn_readlane(my_hi, who); seen0 = __builtin_amdgcn_readlane(my_seen, who);
+        base = __builtin_amdgcn_readlane(my_base, who); len = __builtin_amdgcn_readlane(my_len, who);
+        units = units_of(lo, hi);
+    };
     if (p.runs) {
-        int total = 0;
+        int total = 0, incl = 0;
         for (int b0 = 0; b0 < p.B; b0 += 64) {
-            int l = 0, h = 0, seen;
-            if (b0 + lane < p.B) scored_span(p, b0 + lane, l, h, seen);
-            int n = units_of(l, h) * p.nkv;
+            look(b0);
+            incl = units_of(my_lo, my_hi) * p.nkv;
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-            total += n;
+            for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o); if (lane >= o) incl += up; }
+            total += __builtin_amdgcn_readlane(incl, 63);
         }
-        total = __builtin_amdgcn_readfirstlane(total);
         const int W = max(1, (total + p.nblocks - 1) / p.nblocks), start = blockIdx.x * W, stop = min(total, start + W);
         if (start >= stop && blockIdx.x != 0) return;
         int before = 0, at = -1, at_s = 0;          // units before this group of 64 sequences; the sequence in which the run begins
         for (int b0 = 0; b0 < p.B; b0 += 64) {
-            int l = 0, h = 0, seen;
-            if (b0 + lane < p.B) scored_span(p, b0 + lane, l, h, seen);
-            const int per = units_of(l, h), n = per * p.nkv;
-            int incl = n;
+            if (p.B > 64) {
+                look(b0);
+                incl = units_of(my_lo, my_hi) * p.nkv;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o); if (lane >= o) incl += up; }
-            const int s = before + incl - n;
+                for (int o = 1; o < 64; o <<= 1) { const int up = __shfl_up(incl, o); if (lane >= o) incl += up; }
+            }
+            const int per = units_of(my_lo, my_hi), n = per * p.nkv, s = before + incl - n;
             if (blockIdx.x == 0 && wave == 0 && b0 + lane < p.B)
                 for (int k = 0; k < p.nkv; ++k) {
                     const int a = s + k * per, e = a + per, r0 = a / W, r1 = per ? (e - 1) / W : r0 - 1;
-                    p.meta[(size_t)(b0 + lane) * p.nkv + k] = make_int4(2 * r0 + (a == r0 * W ? 0 : 1), r1 - r0 + 1, l, h);
+                    p.meta[(size_t)(b0 + lane) * p.nkv + k] = make_int4(2 * r0 + (a == r0 * W ? 0 : 1), r1 - r0 + 1, my_lo, my_hi);
                 }
             const uint64_t in = __builtin_amdgcn_ballot_w64(start >= s && start < s + n);
             if (in && at < 0) { const int who = __builtin_ctzll(in); at = b0 + who; at_s = __builtin_amdgcn_readlane(s, who); }
@@ -141,16 +148,16 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
         }
         if (start >= stop) return;
         b = at;
-        scored_span(p, b, lo, hi, seen0);
-        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); seen0 = __builtin_amdgcn_readfirstlane(seen0);
-        units = units_of(lo, hi);
+        take(b);
         kh = (start - at_s) / units;
         u = start - at_s - kh * units;
         u1 = u + stop - start;
     } else {
         b = blockIdx.x / p.nkv; kh = blockIdx.x - b * p.nkv;
-        scored_span(p, b, lo, hi, seen0);
+        scored_rows_of(p, b, base, len);
+        scored_span(p, base, len, lo, hi, seen0);
         lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); seen0 = __builtin_amdgcn_readfirstlane(seen0);
+        base = __builtin_amdgcn_readfirstlane(base); len = __builtin_amdgcn_readfirstlane(len);
         units = units_of(lo, hi); u = 0; u1 = units;
         if (tid == 0) p.meta[blockIdx.x] = make_int4(0, units ? 1 : 0, lo, hi);
     }
@@ -159,15 +166,20 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
     while (u1 > 0) {                                // segments: units [u, min(u1, units)) of pair (b, kh)
         const int stop_u = min(u1, units);
         const bool whole = u == 0 && stop_u == units;
-        int base, len;
-        scored_rows_of(p, b, base, len);
-        base = __builtin_amdgcn_readfirstlane(base); len = __builtin_amdgcn_readfirstlane(len);
         const int ncol = len * p.G;
         const int pstart = lo + u * UNIT, pend = min(hi, lo + stop_u * UNIT);
         const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
         const size_t pair = (size_t)b * p.nkv + kh;
         const int ref = p.slopes ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, hi)) : 0;
 
+        // the first groups' block ids are asked for together with the queries
+        const int last16 = (hi - 1) & ~15;
+        int idv = 0;                                // block ids of 32 groups' units, a lane each
+        auto ids_of = [&](int i) {
+            const int t = min(pstart + wave * 32 + (i + (lane >> 1)) * UNIT + (lane & 1) * 16, last16);
+            idv = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
+        };
+        ids_of(0);
         u32x4 qf[NT][NSTEP];
         int c_lo[NT], c_hi[NT];
         float slope2[NT];
@@ -202,15 +214,13 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
             for (int db = 0; db < NDB; ++db) o[c][db] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
         // A stage: 32 tokens as two units of 16, each inside one page; units behind the last seen slot read that one's again (masked).
-        const int last16 = (hi - 1) & ~15;
         auto page_of = [&](int t) { return (int)__builtin_amdgcn_readfirstlane((int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)); };
         const uint32_t head_bytes = (uint32_t)(p.page * HD * ES);
-        int idv = 0;                                // block ids of 32 groups' units, a lane each: one load (which waits for the ring once) in 32
         auto issue = [&](int i, int buf) {
             const int tb = pstart + wave * 32 + i * UNIT;
-            if ((i & 31) == 0) {
-                const int t = min(tb + (lane >> 1) * UNIT + (lane & 1) * 16, last16);
-                idv = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
+            if ((i & 31) == 0 && i > 0) {
+                ids_of(i);
+                wait_vm<0>();                       // here, where it is rare: left to the compiler the wait, for everything in flight, stands in every round
             }
             const int ids[2] = {__builtin_amdgcn_readlane(idv, (i & 31) * 2), __builtin_amdgcn_readlane(idv, (i & 31) * 2 + 1)};
             const uint32_t to = __builtin_amdgcn_readfirstlane(ring0 + buf * R::STAGE);
@@ -412,9 +422,7 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
             kh = 0;
             do {
                 if (++b >= p.B) return;             // cannot be: the run ends inside the last sequence
-                scored_span(p, b, lo, hi, seen0);
-                lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); seen0 = __builtin_amdgcn_readfirstlane(seen0);
-                units = units_of(lo, hi);
+                take(b);
             } while (units == 0);
         }
     }
@@ -536,15 +544,18 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
 // 16 (i / 2) + 8 half + 4 (i & 1) + r for row 8 i + 4 half + r: what a lane then holds of its column are two runs of eight keys, the second product's operand as it stands.
 // Keys and values come 64 at a time through LDS for all waves: by DMA, two steps ahead of the products with one barrier a step (three stages), or, 8 bits, through registers, which widen them
 // once for all waves.  A key's 16-byte pieces are swizzled by its low bits, a channel's 16 tokens lie side by side: no bank conflicts in either product's reads.
+// What the weights' pass needs of a column.
+struct Col { float m, inv, slope2; int ref, lo, hi, pad0, pad1; };
+static_assert(sizeof(Col) == 32, "two 16-byte loads");
 struct ChunkParams : ScoredParams {
     float*  tmp_out;       // [parts][nkv][rows G][hd] (parts > 1)
     float4* tmp_ml;        // [parts][nkv][rows G]: maximum, sum, the reference of biases
-    float4* ml_all;        // [nkv][rows G]: maximum, 1 / sum, the reference, of every column (with weights)
+    Col*    cols;          // [nkv][rows G] (with weights)
+    float*  shares;        // [splits][B][nkv][max_seq] (splits > 1)
+    int*    reach;         // [B], behind the shares
     int     tiles, parts;  // column tiles of the longest sequence, parts of the keys
     uint32_t g_magic;      // 2^32 / G + 1
 };
-// the same for columns of queries, which lanes read one after the other
-template <int CK> __device__ __forceinline__ int swizzle_q(int c) { return c & (CK - 1); }
 // a key's swizzle: distinct over the keys that eight (rows of 128 bytes) or sixteen (256) neighbouring lanes read
 template <int CK> __device__ __forceinline__ int swizzle_of(int t) { return CK == 16 ? t & 15 : (t & 3) | (t >> 3 & 1) << 2; }
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -552,10 +563,26 @@ template <bool BF> __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f3
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else              return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+// a commutative combination, in which a value may count twice, over lanes 0 to 31 and 32 to 63 each, without LDS
+template <class F> __device__ __forceinline__ int row32(int v, F&& f) {
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));      // lanes' neighbours in fours: 1 0 3 2
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));      // 2 3 0 1
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));     // eights mirrored
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));     // sixteens mirrored
+    float a, c;
+    swap16(__builtin_bit_cast(float, v), a, c);
+    return f(__builtin_bit_cast(int, a), __builtin_bit_cast(int, c));
+}
+// a barrier for what lies in LDS: loads from memory and DMA stay in flight (__syncthreads waits for them)
+__device__ __forceinline__ void lds_barrier() {
+    wait_vm<63>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 enum { FORM_PLAIN, FORM_CAP, FORM_BIAS };           // FORM_BIAS: capped or not
 
 template <int HD, bool INT8, int NW> struct Stage {
-    static constexpr int KEYS = 64, KB = KEYS * HD * 2, BYTES = 2 * KB + (INT8 ? 2 * KEYS * 4 : 0), N = INT8 ? 2 : 3, LDS = N * BYTES + 64;
+    static constexpr int KEYS = 64, KB = KEYS * HD * 2, BYTES = 2 * KB + (INT8 ? 2 * KEYS * 4 : 0), N = INT8 || (HD == 128 && NW < 8) ? 2 : 3, LDS = N * BYTES + 64;
 };
 
 template <int HD, bool INT8, bool BF, int FORM, int NW>
@@ -581,47 +608,24 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
     scored_interval(p, row, lo, hi);
     if (!ok) lo = hi = 0;
     const bool seen = hi > lo;
-    if (tid == 0) { lim[0] = 0x7fffffff; lim[1] = 0; }
-    __syncthreads();
-    // [wlo, whi): what some column of the wave sees; [ilo, ihi): what all do (columns that see nothing do not count)
-    int wlo = seen ? lo : 0x7fffffff, whi = hi, ilo = lo, ihi = seen ? hi : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        wlo = min(wlo, __shfl_xor(wlo, o)); whi = max(whi, __shfl_xor(whi, o));
-        ilo = max(ilo, __shfl_xor(ilo, o)); ihi = min(ihi, __shfl_xor(ihi, o));
-    }
-    if (lane == 0) { atomicMin(&lim[0], wlo); atomicMax(&lim[1], whi); }
-    __syncthreads();
-    wlo = __builtin_amdgcn_readfirstlane(wlo); whi = __builtin_amdgcn_readfirstlane(whi); ilo = __builtin_amdgcn_readfirstlane(ilo); ihi = __builtin_amdgcn_readfirstlane(ihi);
-    const int seen0 = __builtin_amdgcn_readfirstlane(lim[0]), khi = __builtin_amdgcn_readfirstlane(lim[1]), klo = khi > 0 ? seen0 & ~63 : 0;
-    const int all = (khi - klo + 63) / 64, s0 = (int)((long)all * part / p.parts), s1 = (int)((long)all * (part + 1) / p.parts);     // this part's steps
-
     u32x4 qf[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + (size_t)row * p.ldq + h * HD + s * 16 + half * 8);
-        if (!ok) qf[s] = u32x4{0u, 0u, 0u, 0u};
-    }
-    const int ref = FORM == FORM_BIAS && khi > 0 ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, khi)) : 0;
-    const float slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
-    f32x16 o[NDB];
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = NEG_BIG, l = 0.f;
-
+    for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + (size_t)row * p.ldq + h * HD + s * 16 + half * 8);
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
-    const int last16 = khi > 0 ? (khi - 1) & ~15 : 0;
+    int idv = 0;                                    // block ids of 16 steps' units of 16 keys, a lane each
+    auto ids_of = [&](int t0, int last) {
+        const int t = min(t0 + lane * 16, last);
+        idv = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
+        wait_vm<0>();                               // here, where it is rare: left to the compiler the wait, for everything in flight, stands in every step
+    };
+    // Where the walk begins is known before what the rows see is where that starts at slot 0: the first stages are then on their way during the reductions below (what they read behind the
+    // last seen slot, inside the pool, is masked).
+    const bool early = !INT8 && !p.begin && p.parts == 1;
+    if (early) ids_of(0, (p.max_seq - 1) & ~15);
     auto page_of = [&](int t) { return (int)__builtin_amdgcn_readfirstlane((int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)); };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ch_sm;
-    int idv = 0;                                    // block ids of 16 steps' units of 16 keys, a lane each
-    auto ids_for = [&](int st) {
-        if (((st - s0) & 15) == 0) {
-            const int t = min(klo + st * 64 + lane * 16, last16);
-            idv = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
-        }
-    };
+    int klo = 0, s0 = 0, last16 = (p.max_seq - 1) & ~15;
+    auto ids_for = [&](int st) { if (((st - s0) & 15) == 0 && !(early && st == s0)) ids_of(klo + st * 64, last16); };
     // base of a unit's keys and values; a unit past the last seen slot is that one's again (masked)
     const uint32_t head_elems = (uint32_t)(p.page * HD);
     auto unit_at = [&](int st, int u, int& ti, uint32_t& hk) {
@@ -651,6 +655,30 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             dma16(to + KB, voff, kb + (uint64_t)(uint32_t)p.nkv * head_elems + (uint32_t)ti + (uint32_t)(d % KU * 32) * (uint32_t)p.page);
         }
     };
+    if constexpr (!INT8) if (early) { issue(0, 0); if (ST::N > 2) issue(1, 1); }
+    // [wlo, whi): what some column of the wave sees; [ilo, ihi): what all do (columns that see nothing do not count)
+    if (tid == 0) { lim[0] = 0x7fffffff; lim[1] = 0; }
+    lds_barrier();
+    const int wlo = __builtin_amdgcn_readfirstlane(row32(seen ? lo : 0x7fffffff, [](int a, int c) { return min(a, c); })), whi = __builtin_amdgcn_readfirstlane(row32(hi, [](int a, int c) { return max(a, c); }));
+    const int ilo = __builtin_amdgcn_readfirstlane(row32(lo, [](int a, int c) { return max(a, c); })), ihi = __builtin_amdgcn_readfirstlane(row32(seen ? hi : 0x7fffffff, [](int a, int c) { return min(a, c); }));
+    if (lane == 0) { atomicMin(&lim[0], wlo); atomicMax(&lim[1], whi); }
+    lds_barrier();
+    const int seen0 = __builtin_amdgcn_readfirstlane(lim[0]), khi = __builtin_amdgcn_readfirstlane(lim[1]);
+    klo = khi > 0 ? seen0 & ~63 : 0;
+    const int all = (khi - klo + 63) / 64, s1 = (int)((long)all * (part + 1) / p.parts);           // this part's steps
+    s0 = (int)((long)all * part / p.parts);
+    last16 = khi > 0 ? (khi - 1) & ~15 : 0;
+    const int ref = FORM == FORM_BIAS && khi > 0 ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, khi)) : 0;
+    const float slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
+    f32x16 o[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = NEG_BIG, l = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+        if (!ok) qf[s] = u32x4{0u, 0u, 0u, 0u};
     // ---- 8 bits: 16-byte pieces through registers, a thread takes the same piece numbers of every stage
     constexpr int PIECES = 64 * HD / 16, JP = INT8 ? (PIECES + 64 * NW - 1) / (64 * NW) : 1;
     u32x4 rk[JP], rv[JP];
@@ -671,6 +699,8 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             const int t = min(klo + st * 64 + (tid & 63 & ~15), last16), blk = __shfl(idv, ((st - s0) & 15) * 4 + ((tid & 63) >> 4));
             const size_t hk = (size_t)min(max(blk, 0), p.num_blocks - 1) * 2 * p.nkv + kh + (tid >= 64 ? p.nkv : 0);
             rs = p.scale_base[hk * p.page + t % p.page + (tid & 15)];
+            const int key = klo + st * 64 + (tid & 63);
+            if (key >= khi || key < seen0) rs = 0.f;    // whatever the pool holds there
         }
     };
     auto store8 = [&](int buf) {
@@ -685,122 +715,141 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             *reinterpret_cast<u32x4*>(st + KB + i * 32) = widen_codes<BF>(rv[j][0], rv[j][1]);
             *reinterpret_cast<u32x4*>(st + KB + i * 32 + 16) = widen_codes<BF>(rv[j][2], rv[j][3]);
         }
-        if (tid < 128) reinterpret_cast<float*>(st + 2 * KB)[tid] = rs;
+        if (tid < 128) reinterpret_cast<float*>(st + 2 * KB)[tid] = rs;              // 0 for a slot that no row here sees (fetch8)
     };
 
     // where the lane's fragments lie: its key in a group of 32, that key's pieces
     const int kt = 16 * (col >> 4) + 8 * (col >> 2 & 1) + 4 * (col >> 3 & 1) + (col & 3), kf = swizzle_of<CK>(kt & 15);
-    auto compute = [&](const char* st, int t0, auto masked_c) {
-        constexpr bool MASKED = decltype(masked_c)::value;
-        float sv[2][16];
+    // A step's 64 keys as two groups of 32.  The fragments are asked for a phase ahead of their use (the second group's keys and the first one's values before the first softmax): read where
+    // they are used, every product waited for its own.
+    auto read_keys = [&](const char* st, int g, u32x4 (&f)[KS]) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            f32x16 s;
+        for (int ks = 0; ks < KS; ++ks) f[ks] = *reinterpret_cast<const u32x4*>(st + (g * 32 + kt) * ROW + (((ks * 2 + half) ^ kf) << 4));
+    };
+    auto read_values = [&](const char* st, int g, u32x4 (&f)[2][NDB]) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-                s = mfma32<BF>(*reinterpret_cast<const u32x4*>(st + (g * 32 + kt) * ROW + (((ks * 2 + half) ^ kf) << 4)), qf[ks], s);
+            for (int d = 0; d < NDB; ++d) f[k][d] = *reinterpret_cast<const u32x4*>(st + KB + ((g * 2 + k) * HD + d * 32 + col) * 32 + half * 16);
+    };
+    auto scores = [&](const u32x4 (&f)[KS], f32x16& s) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sv[g][i] = s[i];
-        }
-        // sv[g][8 kk + e] is key t0 + 32 g + 16 kk + 8 half + e
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mfma32<BF>(f[ks], qf[ks], s);
+    };
+    // scores of a group -> probabilities as the second product's operand; sv[8 kk + e] is key t0 + 16 kk + 8 half + e
+    auto weigh = [&](const f32x16& s, const char* st, int g, int t0, u32x4 (&pf)[2], bool masked) {
+        float sv[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sv[i] = s[i];
         if constexpr (INT8) {
-            const f32x4* sc = reinterpret_cast<const f32x4*>(st + 2 * KB) + half * 2;
+            const f32x4* sc = reinterpret_cast<const f32x4*>(st + 2 * KB) + g * 8 + half * 2;
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) sv[g][i] *= sc[g * 8 + (i >> 3) * 4 + (i >> 2 & 1)][i & 3];
+            for (int i = 0; i < 16; ++i) sv[i] *= sc[(i >> 3) * 4 + (i >> 2 & 1)][i & 3];
         }
         float mul = p.scale1;                       // scores are sv times mul from here on
         if constexpr (FORM != FORM_PLAIN) {
             if (FORM == FORM_CAP || p.capped) {
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sv[g][i] *= p.scale1;
-                    tanh_all(sv[g]);
-                }
+                for (int i = 0; i < 16; ++i) sv[i] *= p.scale1;
+                tanh_all(sv);
                 mul = p.cap_log2;
             }
         }
         if constexpr (FORM == FORM_BIAS) {
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int t = t0 + g * 32 + (k >> 1) * 16 + half * 8 + (k & 1) * 4;
-                    i32x4 kp = {t - ref, t + 1 - ref, t + 2 - ref, t + 3 - ref};
-                    if (p.key_pos) {                // the planes' rows of four tokens lie inside a page
-                        const int tc = min(t, last16 + 12), blk = scored_block(p, bt, tc);
-                        kp = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)blk * p.nkv + kh) * p.page + tc % p.page);
-                        kp -= ref;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sv[g][k * 4 + e] = __builtin_fmaf(slope2, (float)kp[e], sv[g][k * 4 + e] * mul);
+            for (int k = 0; k < 4; ++k) {
+                const int t = t0 + (k >> 1) * 16 + half * 8 + (k & 1) * 4;
+                i32x4 kp = {t - ref, t + 1 - ref, t + 2 - ref, t + 3 - ref};
+                if (p.key_pos) {                    // the planes' rows of four tokens lie inside a page
+                    const int tc = min(t, last16 + 12), blk = scored_block(p, bt, tc);
+                    kp = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)blk * p.nkv + kh) * p.page + tc % p.page);
+                    kp -= ref;
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sv[k * 4 + e] = __builtin_fmaf(slope2, (float)kp[e], sv[k * 4 + e] * mul);
+            }
             mul = 1.f;
+        }
+        if (masked) {
+            const int a = lo - t0 - half * 8, e = hi - t0 - half * 8;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sv[i] = (i >> 3) * 16 + (i & 7) >= a && (i >> 3) * 16 + (i & 7) < e ? sv[i] : -__builtin_inff();
         }
         float mx = -__builtin_inff();
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if (MASKED) {
-                    const int t = t0 + g * 32 + (i >> 3) * 16 + half * 8 + (i & 7);
-                    sv[g][i] = t >= lo && t < hi ? sv[g][i] : -__builtin_inff();
-                }
-                mx = fmaxf(mx, sv[g][i]);
-            }
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sv[i]);
         mx = fmaxf(xor32_max(mx) * mul, NEG_BIG);
         if (__builtin_amdgcn_ballot_w64(mx > m + DEFER)) {
-            const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
+            const float mn = fmaxf(m, mx);
+            float alpha = __builtin_amdgcn_exp2f(m - mn);
             l *= alpha;
+            // In place, by hand: as plain products the compiler keeps all outputs twice, before and after, copies one over the other and spills.  It does not see what the statements read, so
+            // the wait states between a product's issue and a read of its result (11 for the 8 passes of these), and from there to the next product, stand here.
+            asm volatile("s_nop 15\n\ts_nop 7" : "+v"(alpha));
 #pragma unroll
-            for (int d = 0; d < NDB; ++d) o[d] *= alpha;
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[d][i]) : "v"(alpha));
+            asm volatile("s_nop 7");
             m = mn;
         }
         float psum = 0.f;
-        u32x4 pf[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k) {
             float pe[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                pe[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[k >> 1][(k & 1) * 8 + e], mul, -m));
+                pe[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[k * 8 + e], mul, -m));
                 psum += pe[e];
                 if constexpr (INT8) {
-                    const float vs = (reinterpret_cast<const float*>(st + 2 * KB) + 64)[k * 16 + half * 8 + e] * VS;
-                    const int t = t0 + k * 16 + half * 8 + e;
-                    pe[e] = !MASKED || (t >= lo && t < hi) ? pe[e] * vs : 0.f;
+                    const float vs = (reinterpret_cast<const float*>(st + 2 * KB) + 64)[g * 32 + k * 16 + half * 8 + e] * VS;
+                    pe[e] *= vs;
                 }
             }
             pf[k] = act_pack8<BF>(pe);
         }
         l += psum;
+    };
+    auto add = [&](u32x4 (&f)[2][NDB], const u32x4 (&pf)[2], int t0) {
+        if (!INT8 && (t0 + 32 > khi || t0 < seen0)) {        // slots that no row here sees may hold anything, NaN too: their weights are zero, their values are made so
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int d = 0; d < NDB; ++d) {
-                u32x4 a = *reinterpret_cast<const u32x4*>(st + KB + (k * HD + d * 32 + col) * 32 + half * 16);
-                if (MASKED && !INT8 && (t0 + 64 > khi || t0 < seen0)) {     // slots that no row here sees may hold anything, NaN too: their weights are zero, their values are made so
-                    const int t = t0 + k * 16 + half * 8;
+                for (int w = 0; w < 4; ++w) {
+                    const int t = t0 + k * 16 + half * 8 + w * 2;
+                    const uint32_t keep = (t < khi && t >= seen0 ? 0xFFFFu : 0u) | (t + 1 < khi && t + 1 >= seen0 ? 0xFFFF0000u : 0u);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (t + e >= khi || t + e < seen0) a[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+                    for (int d = 0; d < NDB; ++d) f[k][d][w] &= keep;
                 }
-                o[d] = mfma32<BF>(a, pf[k], o[d]);
-            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) o[d] = mfma32<BF>(f[k][d], pf[k], o[d]);
     };
     auto step = [&](const char* st, int t0) {
         if (t0 >= whi || t0 + 64 <= wlo) return;
-        if (t0 >= ilo && t0 + 64 <= ihi) compute(st, t0, std::false_type{});
-        else compute(st, t0, std::true_type{});
+        const bool masked = t0 < ilo || t0 + 64 > ihi;
+        u32x4 kf0[KS], kf1[KS], vf[2][NDB], pf[2];
+        f32x16 s;
+        read_keys(st, 0, kf0);
+        scores(kf0, s);
+        read_keys(st, 1, kf1);
+        read_values(st, 0, vf);
+        asm volatile("" ::: "memory");
+        weigh(s, st, 0, t0, pf, masked);
+        scores(kf1, s);
+        add(vf, pf, t0);
+        read_values(st, 1, vf);
+        asm volatile("" ::: "memory");
+        weigh(s, st, 1, t0 + 32, pf, masked);
+        add(vf, pf, t0 + 32);
     };
-    wait_vm<0>();                                   // the queries are here: no wait for them inside the loop
     if constexpr (!INT8) {
         constexpr int NS = ST::N;
-        for (int i = 0; i < min(NS - 1, s1 - s0); ++i) issue(s0 + i, i);
+        if (!early) for (int i = 0; i < min(NS - 1, s1 - s0); ++i) issue(s0 + i, i);
         int buf = 0;
         for (int st = s0; st < s1; ++st) {
             if (st + 1 < s1) wait_vm<2 * JK * (NS - 2)>(); else wait_vm<0>();        // this step's loads of this wave (the next step's may be left)
@@ -810,6 +859,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             step(ch_sm + buf * ST::BYTES, klo + st * 64);
             buf = buf == NS - 1 ? 0 : buf + 1;
         }
+        if (early && s0 == s1) wait_vm<0>();        // nothing is seen: what was asked for early must not land in LDS that is another block's by then
     } else if (s0 < s1) {
         fetch8(s0);
         store8(0);
@@ -850,7 +900,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
         }
     if (half == 0) {
         if (p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, seen, seen ? scored_shift(p, row, h, ref) : 0.f);
-        if (p.ml_all) p.ml_all[at] = make_float4(m, scored_inv(l, seen), __builtin_bit_cast(float, ref), 0.f);
+        if (p.cols) p.cols[at] = Col{m, scored_inv(l, seen), slope2, ref, seen ? lo : 0, seen ? hi : 0, 0, 0};
     }
 }
 
@@ -896,166 +946,174 @@ __global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) 
     for (int k = 0; k < CPL; ++k) dst[k] = act_to_bits<BF>(seen ? acc[k] * inv : 0.f);
     if (lane == 0) {
         if (p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, seen, seen ? scored_shift(p, row, h, ref) : 0.f);
-        if (p.ml_all) p.ml_all[at] = make_float4(m, inv, __builtin_bit_cast(float, ref), 0.f);
+        if (p.cols) p.cols[at] = Col{m, inv, p.slopes ? p.slopes[h] * kLog2e : 0.f, ref, a, e, 0, 0};
     }
 }
 
-// The weights of many rows: S^T once more, a wave's 32 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 128 keys, its 16 waves four groups of 32
-// columns of each 128 at a time; a probability is added in the lane of its column, lanes and groups meet once at the end: no atomics, the same sums every time.
+// The weights of many rows: S^T once more, a wave's 64 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 256 keys, its 8 waves the two halves of
+// 128 columns at a time (three stages of DMA); a probability is added in the lane of its column, lanes and halves meet once at the end: no atomics, the same sums every time.  Keys that
+// all rows see take longer than late ones: where blocks are few the columns are dealt to `splits` blocks and scored_decay_kernel adds their shares.
 template <int HD, bool INT8, bool BF, int FORM>
-__global__ __launch_bounds__(1024) void scored_sums_kernel(const ChunkParams p, int key_tiles) {
-    constexpr int KS = HD / 16, ROW = HD * 2, CK = ROW / 16, QB = 128 * ROW, LOADS = QB / 1024, JL = LOADS / 16;
+__global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p, int key_tiles, int splits) {
+    constexpr int KS = HD / 16, ROW = HD * 2, CK = ROW / 16, QB = 128 * ROW, SB = QB + 4096, LOADS = QB / 1024, JL = LOADS / 8, NS = 3;
     extern __shared__ __attribute__((aligned(16))) char su_sm[];
-    struct Col { float m, inv, slope2; int ref, lo, hi, pad0, pad1; };
-    static_assert(sizeof(Col) == 32, "");
-    Col* cols = reinterpret_cast<Col*>(su_sm + 2 * QB);              // [2][128]
-    float* meet = reinterpret_cast<float*>(su_sm);                   // [3][128], over the columns when they are done
-    int* s_reach = reinterpret_cast<int*>(su_sm + 2 * QB + 2 * 128 * sizeof(Col));
+    float* meet = reinterpret_cast<float*>(su_sm);                   // [256], over the columns when they are done
+    int* s_reach = reinterpret_cast<int*>(su_sm + NS * SB);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5, cg = wave >> 2;
     int id = blockIdx.x;
-    const int tile = id % key_tiles; id /= key_tiles;
-    const int kh = id % p.nkv, b = id / p.nkv;
+    const int tile = id % key_tiles; id /= key_tiles;                // early keys, which most rows see, first
+    const int kh = id % p.nkv; id /= p.nkv;
+    const int b = id % p.B, split = id / p.B;
     int base, len;
     scored_rows_of(p, b, base, len);
-    const int ncol = len * p.G, tw = tile * 128 + (wave & 3) * 32;    // the wave's first slot
-    if (tid == 0) *s_reach = 0;
-    __syncthreads();
-    int reach = 0;
-    for (int i = tid; i < len; i += 1024) { int a, e; scored_interval(p, base + i, a, e); reach = max(reach, e); }
+    const int ncol = len * p.G, tw = tile * 256 + (wave & 3) * 64;    // the wave's first slot
+    const int all = (ncol + 127) / 128, st0 = (int)((long)all * split / splits), st1 = (int)((long)all * (split + 1) / splits);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)su_sm;
+    const char* cols = reinterpret_cast<const char*>(p.cols + (size_t)kh * p.rows * p.G + (size_t)base * p.G);
+    auto issue = [&](int st, int buf) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) reach = max(reach, __shfl_xor(reach, o));
-    if (lane == 0) atomicMax(s_reach, reach);
-    __syncthreads();
+        for (int j = 0; j < JL; ++j) {
+            const int d = j * 8 + wave, cl = d * (1024 / ROW) + lane / CK, c = min(st * 128 + cl, ncol - 1);
+            const int r = p.G == 1 ? c : (int)(((unsigned long long)(unsigned)c * p.g_magic) >> 32);
+            dma16(__builtin_amdgcn_readfirstlane(lds0 + buf * SB + d * 1024), (const uint16_t*)p.q + (size_t)(base + r) * p.ldq + (kh * p.G + c - r * p.G) * HD + ((lane % CK) ^ (cl & (CK - 1))) * 8);
+        }
+        if (wave < 4)                                                // 32 columns' facts a load (the last, past the sequence's, are its last one's: not looked at)
+            dma16(__builtin_amdgcn_readfirstlane(lds0 + buf * SB + QB + wave * 1024), cols + (size_t)min(st * 128 + wave * 32 + (lane >> 1), ncol - 1) * 32 + (lane & 1) * 16);
+    };
+    if (st0 < st1) issue(st0, 0);
+    if (st0 + 1 < st1) issue(st0 + 1, 1);
+    if (tid == 0) *s_reach = 0;
+    lds_barrier();
+    int reach = 0;
+    for (int i = tid; i < len; i += 512) { int a, e; scored_interval(p, base + i, a, e); reach = max(reach, e); }
+    reach = row32(reach, [](int a, int c) { return max(a, c); });
+    if ((lane & 31) == 0) atomicMax(s_reach, reach);
+    lds_barrier();
     reach = __builtin_amdgcn_readfirstlane(*s_reach);
-    if (tile * 128 >= reach) return;
+    if (splits > 1 && tile == 0 && kh == 0 && split == 0 && tid == 0) p.reach[b] = reach;
+    if (tile * 256 >= reach) { wait_vm<0>(); return; }               // the loads above must not land in another block's LDS
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
-    u32x4 kfr[KS];
-    float ksc[INT8 ? 16 : 1];
-    i32x4 kp[FORM == FORM_BIAS ? 4 : 1];
-    {
-        const int t = min(tw + col, reach - 1), blk = scored_block(p, bt, t);
+    u32x4 kfr[2][KS];
+    float ksc[INT8 ? 2 : 1][INT8 ? 16 : 1];
+    i32x4 kp[FORM == FORM_BIAS ? 2 : 1][FORM == FORM_BIAS ? 4 : 1];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int t = min(tw + g * 32 + col, reach - 1), blk = scored_block(p, bt, t);
         const size_t at = (((size_t)blk * 2) * p.nkv + kh) * p.page + t % p.page;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             if constexpr (INT8) {
                 const u32x2 v = *reinterpret_cast<const u32x2*>((const char*)p.kv_base + at * HD + s * 16 + half * 8);
-                kfr[s] = widen_codes<BF>(v[0], v[1]);
-            } else kfr[s] = *reinterpret_cast<const u32x4*>((const uint16_t*)p.kv_base + at * HD + s * 16 + half * 8);
+                kfr[g][s] = widen_codes<BF>(v[0], v[1]);
+            } else kfr[g][s] = *reinterpret_cast<const u32x4*>((const uint16_t*)p.kv_base + at * HD + s * 16 + half * 8);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // the lane's results are keys 8 i + 4 half + r
-            const int tt = tw + i * 8 + half * 4, tc = min(tt, (reach - 1) & ~3), bl = scored_block(p, bt, tc);
+            const int tt = tw + g * 32 + i * 8 + half * 4, tc = min(tt, (reach - 1) & ~3), bl = scored_block(p, bt, tc);
             if constexpr (INT8) {
                 const f32x4 v = *reinterpret_cast<const f32x4*>(p.scale_base + (((size_t)bl * 2) * p.nkv + kh) * p.page + tc % p.page);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) ksc[i * 4 + e] = v[e];
+                for (int e = 0; e < 4; ++e) ksc[INT8 ? g : 0][INT8 ? i * 4 + e : 0] = v[e];
             }
             if constexpr (FORM == FORM_BIAS) {
-                kp[i] = i32x4{tt, tt + 1, tt + 2, tt + 3};
-                if (p.key_pos) kp[i] = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)bl * p.nkv + kh) * p.page + tc % p.page);
+                kp[g][i] = i32x4{tt, tt + 1, tt + 2, tt + 3};
+                if (p.key_pos) kp[g][i] = *reinterpret_cast<const i32x4*>(p.key_pos + ((size_t)bl * p.nkv + kh) * p.page + tc % p.page);
             }
         }
     }
-    float acc[16];
+    float acc[2][16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)su_sm;
-    const int steps = (ncol + 127) / 128;
-    auto place = [&](int c, int& row, int& h) {
-        c = min(c, ncol - 1);
-        const int r = p.G == 1 ? c : (int)(((unsigned long long)(unsigned)c * p.g_magic) >> 32);
-        row = base + r; h = kh * p.G + c - r * p.G;
-    };
-    auto issue = [&](int st, int buf) {
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int j = 0; j < JL; ++j) {
-            const int d = j * 16 + wave, cl = d * (1024 / ROW) + lane / CK;
-            int row, h;
-            place(st * 128 + cl, row, h);
-            dma16(__builtin_amdgcn_readfirstlane(lds0 + buf * QB + d * 1024), (const uint16_t*)p.q + (size_t)row * p.ldq + h * HD + ((lane % CK) ^ swizzle_q<CK>(cl)) * 8);
-        }
-    };
-    Col mine;
-    auto fetch = [&](int st) {
-        if (tid >= 128) return;
-        const int c = st * 128 + tid;
-        int row, h;
-        place(c, row, h);
-        const float4 ml = p.ml_all[(size_t)kh * p.rows * p.G + (size_t)base * p.G + min(c, ncol - 1)];
-        mine.m = ml.x; mine.inv = ml.y; mine.ref = __builtin_bit_cast(int, ml.z);
-        mine.slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
-        scored_interval(p, row, mine.lo, mine.hi);
-        if (c >= ncol) mine.lo = mine.hi = 0;
-    };
-    fetch(0);
-    issue(0, 0);
-    if (tid < 128) cols[tid] = mine;
-    wait_vm<0>();
-    for (int st = 0; st < steps; ++st) {
-        const int buf = st & 1;
-        __syncthreads();
-        if (st + 1 < steps) { issue(st + 1, buf ^ 1); fetch(st + 1); }
-        const Col c = cols[buf * 128 + cg * 32 + col];
-        if (__builtin_amdgcn_ballot_w64(c.lo < tw + 32 && c.hi > tw)) {
-            const bool masked = __builtin_amdgcn_ballot_w64(c.lo > tw || c.hi < tw + 32) != 0;
-            f32x16 s;
+        for (int i = 0; i < 16; ++i) acc[g][i] = 0.f;
+    int buf = 0;
+    const int f = col & (CK - 1);
+    wait_vm<0>();                                                    // the keys are here: no wait for them inside the loop
+    for (int st = st0; st < st1; ++st) {
+        if (st + 1 < st1) { if (wave < 4) wait_vm<JL + 1>(); else wait_vm<JL>(); } else wait_vm<0>();      // all but the next step's loads of this wave
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (st + 2 < st1) issue(st + 2, buf == 0 ? 2 : buf - 1);
+        const char* stage = su_sm + buf * SB;
+        buf = buf == 2 ? 0 : buf + 1;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = 0.f;
-            const int cl = cg * 32 + col, f = swizzle_q<CK>(cl);
-            const char* q = su_sm + buf * QB + cl * ROW;
+        for (int ct = 0; ct < 2; ++ct) {
+            const int cl = cg * 64 + ct * 32 + col;
+            Col c = reinterpret_cast<const Col*>(stage + QB)[cl];
+            if (st * 128 + cl >= ncol) c.lo = c.hi = 0;
+            if (!__builtin_amdgcn_ballot_w64(c.lo < tw + 64 && c.hi > tw)) continue;
+            const bool masked = __builtin_amdgcn_ballot_w64(c.lo > tw || c.hi < tw + 64) != 0;
+            f32x16 s[2];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = mfma32<BF>(kfr[ks], *reinterpret_cast<const u32x4*>(q + (((ks * 2 + half) ^ f) << 4)), s);
-            float sv[16];
+            for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sv[i] = INT8 ? s[i] * ksc[INT8 ? i : 0] : s[i];
-            float mul = p.scale1;
-            if constexpr (FORM != FORM_PLAIN) {
-                if (FORM == FORM_CAP || p.capped) {
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 q = *reinterpret_cast<const u32x4*>(stage + cl * ROW + (((ks * 2 + half) ^ f) << 4));
+                s[0] = mfma32<BF>(kfr[0][ks], q, s[0]);
+                s[1] = mfma32<BF>(kfr[1][ks], q, s[1]);
+            }
+            c.m = fmaxf(c.m, NEG_BIG);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sv[i] *= p.scale1;
-                    tanh_all(sv);
-                    mul = p.cap_log2;
+            for (int g = 0; g < 2; ++g) {
+                float sv[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sv[i] = INT8 ? s[g][i] * ksc[INT8 ? g : 0][INT8 ? i : 0] : s[g][i];
+                float mul = p.scale1;
+                if constexpr (FORM != FORM_PLAIN) {
+                    if (FORM == FORM_CAP || p.capped) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sv[i] *= p.scale1;
+                        tanh_all(sv);
+                        mul = p.cap_log2;
+                    }
                 }
-            }
-            if constexpr (FORM == FORM_BIAS) {
+                if constexpr (FORM == FORM_BIAS) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sv[i] = __builtin_fmaf(c.slope2, (float)(kp[i >> 2][i & 3] - c.ref), sv[i] * mul);
-                mul = 1.f;
-            }
-            if (!masked) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], mul, -c.m)), c.inv, acc[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int t = tw + (i >> 2) * 8 + half * 4 + (i & 3);
-                    const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], mul, -c.m)) * c.inv;
-                    acc[i] += t >= c.lo && t < c.hi ? pe : 0.f;
+                    for (int i = 0; i < 16; ++i) sv[i] = __builtin_fmaf(c.slope2, (float)(kp[g][i >> 2][i & 3] - c.ref), sv[i] * mul);
+                    mul = 1.f;
                 }
+                if (masked) {                                        // a column that sees nothing: exp(-inf) = 0 of each
+                    const int a = c.lo - tw - g * 32 - half * 4, e = c.hi - tw - g * 32 - half * 4;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sv[i] = (i >> 2) * 8 + (i & 3) >= a && (i >> 2) * 8 + (i & 3) < e ? sv[i] : -__builtin_inff();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[g][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(sv[i], mul, -c.m)), c.inv, acc[g][i]);
             }
-        }
-        if (st + 1 < steps) {
-            if (tid < 128) cols[(buf ^ 1) * 128 + tid] = mine;
-            wait_vm<0>();
         }
     }
-    float sum = 0.f;                                                 // lane `col` < 16 ends up with result `col`
+    float sum = 0.f;                                                 // lane `col` ends up with result `col`: 16 of each group
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float v = acc[i];
+    for (int i = 0; i < 32; ++i) {
+        float v = acc[i >> 4][i & 15];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) v += __shfl_xor(v, o);
         if (col == i) sum = v;
     }
     __syncthreads();
-    const int key = (wave & 3) * 32 + (col >> 2) * 8 + half * 4 + (col & 3);
-    if (cg > 0 && col < 16) meet[(cg - 1) * 128 + key] = sum;
+    const int key = (wave & 3) * 64 + (col >> 4) * 32 + (col >> 2 & 3) * 8 + half * 4 + (col & 3);
+    if (cg > 0) meet[key] = sum;
     __syncthreads();
-    if (cg > 0 || col >= 16) return;
-    sum += meet[key]; sum += meet[128 + key]; sum += meet[256 + key];
-    const int t = tile * 128 + key;
+    if (cg > 0) return;
+    sum += meet[key];
+    const int t = tile * 256 + key;
     if (t >= reach) return;
+    if (splits > 1) {
+        p.shares[(((size_t)split * p.B + b) * p.nkv + kh) * p.max_seq + t] = sum;
+        return;
+    }
     const int blk = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
+    if (blk < 0 || blk >= p.num_blocks) return;
+    float* to = p.weights + ((size_t)blk * p.nkv + kh) * p.page + t % p.page;
+    *to = scored_decayed(p, *to, sum);
+}
+
+__global__ __launch_bounds__(256) void scored_decay_kernel(const ChunkParams p, int splits) {
+    const int b = blockIdx.z, kh = blockIdx.y, t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= p.reach[b]) return;
+    float sum = 0.f;
+    for (int i = 0; i < splits; ++i) sum += p.shares[(((size_t)i * p.B + b) * p.nkv + kh) * p.max_seq + t];
+    const int blk = p.block_table[(size_t)b * p.max_blocks + (int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
     if (blk < 0 || blk >= p.num_blocks) return;
     float* to = p.weights + ((size_t)blk * p.nkv + kh) * p.page + t % p.page;
     *to = scored_decayed(p, *to, sum);
@@ -1066,11 +1124,11 @@ __global__ __launch_bounds__(1024) void scored_sums_kernel(const ChunkParams p, 
 struct Plan {
     bool   few;                // the few-row kernel: at most 32 (row, head) pairs of a key/value head a sequence
     int    nblocks, ncol, ctx_pad, runs;
-    int    waves, tiles, parts;                                  // the many-row kernel
+    int    waves, tiles, parts, splits;                          // the many-row kernels
     size_t tmp_out, tmp_ml, ml_all, spill, meta, bytes;          // offsets; bytes: all
 };
 constexpr int RUNS = 256;      // one block of the few-row kernel a compute unit
-Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, bool track) {
+Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, bool track, bool int8) {
     Plan pl{};
     const int G = nh / nkv;
     size_t at = 0;
@@ -1086,12 +1144,20 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         if (track) { pl.ml_all = region(pairs * pl.ncol * 8); pl.spill = region(pairs * pl.ncol * pl.ctx_pad * 4); }
     } else {
         const long cols = (long)q_len * G;
-        pl.waves = cols <= 64 ? 2 : cols <= 128 ? 4 : 8;
+        // Four waves a block, two blocks a compute unit: one fills in while the other one starts, ends or waits.  us by eight / by four: 16 x 64 rows 12.8 / 10.4, 4 x 512 34 / 30, 32 x 512
+        // 154 / 139, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 895 / 952) and
+        // where keys and values are widened on the way (333 rows behind 3001 46 / 53).
+        pl.waves = cols <= 64 ? 2 : cols <= 128 || (!int8 && max_seq < 8192) ? 4 : 8;
         pl.tiles = (int)((cols + 32 * pl.waves - 1) / (32 * pl.waves));
         const long blocks = (long)pl.tiles * B * nkv, room = 256 * 8 / pl.waves;
         pl.parts = (int)std::max(1l, std::min({room / std::max(1l, blocks), (max_seq + 255l) / 256, 64l}));
         if (pl.parts > 1) { pl.tmp_out = region((size_t)pl.parts * rows * nh * hd * 4); pl.tmp_ml = region((size_t)pl.parts * rows * nh * 16); }
-        if (track) pl.ml_all = region((size_t)rows * nh * 16);
+        if (track) {
+            pl.ml_all = region((size_t)rows * nh * sizeof(Col));
+            const long kb = (long)cdiv(max_seq, 256) * nkv * B;
+            pl.splits = (int)std::max(1l, std::min({512 / kb, (cols + 1023) / 1024, 4l}));
+            if (pl.splits > 1) pl.spill = region(((size_t)pl.splits * nkv * max_seq + 1) * B * 4);
+        }
     }
     pl.bytes = at;
     return pl;
@@ -1121,8 +1187,9 @@ int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
     if (rc != MI355_OK) return rc;
     if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 3) / 4)), dim3(256), 0, st, c);
     if (c.weights) {
-        const int key_tiles = cdiv(c.max_seq, 128);
-        rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 2 * 128 * HD * 2 + 2 * 128 * 32 + 16, 1024, (long)key_tiles * c.nkv * c.B, key_tiles);
+        const int key_tiles = cdiv(c.max_seq, 256);
+        rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 3 * (128 * HD * 2 + 4096) + 16, 512, (long)key_tiles * c.nkv * c.B * pl.splits, key_tiles, pl.splits);
+        if (rc == MI355_OK && pl.splits > 1) hipLaunchKernelGGL(scored_decay_kernel, dim3(cdiv(c.max_seq, 256), c.nkv, c.B), dim3(256), 0, st, c, pl.splits);
     }
     return rc;
 }
@@ -1135,7 +1202,7 @@ int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
 
 extern "C" size_t mi355_paged_attn_scored_workspace_bytes(int32_t B, int32_t q_len, int32_t rows, int32_t nh, int32_t nkv, int32_t hd, int32_t max_seq_len, int32_t track) {
     if (B <= 0 || q_len <= 0 || rows <= 0 || nh <= 0 || nkv <= 0 || nh % nkv || hd <= 0 || max_seq_len <= 0) return 0;
-    return plan_of(B, q_len, rows, nh, nkv, hd, max_seq_len, track != 0).bytes;
+    return std::max(plan_of(B, q_len, rows, nh, nkv, hd, max_seq_len, track != 0, false).bytes, plan_of(B, q_len, rows, nh, nkv, hd, max_seq_len, track != 0, true).bytes);
 }
 
 extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_kv_layer_t* kv, const int32_t* block_table, int32_t max_blocks_per_seq,
@@ -1145,7 +1212,7 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
     DecodeParams p;
     const int rc = scored_params(p, q, ldq, kv, block_table, max_blocks_per_seq, row_start, B, q_len, rows, nh, score, max_seq_len, out, lse, weights, decay);
     if (rc != MI355_OK) return rc;
-    const Plan pl = plan_of(B, q_len, rows, nh, kv->nkv, kv->hd, max_seq_len, weights != nullptr);
+    const Plan pl = plan_of(B, q_len, rows, nh, kv->nkv, kv->hd, max_seq_len, weights != nullptr, kv->kv_dtype == MI355_KV_INT8);
     if (pl.bytes && (pl.bytes > workspace_bytes || !workspace)) {
         mi355_set_error("paged_attn_scored: workspace %zu < %zu", workspace_bytes, pl.bytes);
         return MI355_ERR_WORKSPACE;
@@ -1178,8 +1245,9 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
     static_cast<ScoredParams&>(c) = p;
     c.tiles = pl.tiles; c.parts = pl.parts; c.g_magic = (uint32_t)((1ull << 32) / (unsigned)p.G + 1);
     c.tmp_out = pl.parts > 1 ? (float*)(ws + pl.tmp_out) : nullptr; c.tmp_ml = pl.parts > 1 ? (float4*)(ws + pl.tmp_ml) : nullptr;
-    c.ml_all = weights ? (float4*)(ws + pl.ml_all) : nullptr;
-    MI355_CHECK_ARG((long)pl.tiles * B * kv->nkv * pl.parts < (1l << 31) && (long)cdiv(max_seq_len, 128) * kv->nkv * B < (1l << 31) && (long)q_len * p.G * p.G < (1l << 32),
+    c.cols = weights ? (Col*)(ws + pl.ml_all) : nullptr; c.shares = weights && pl.splits > 1 ? (float*)(ws + pl.spill) : nullptr;
+    c.reach = c.shares ? (int*)(c.shares + (size_t)pl.splits * B * kv->nkv * max_seq_len) : nullptr;
+    MI355_CHECK_ARG((long)pl.tiles * B * kv->nkv * pl.parts < (1l << 31) && (long)cdiv(max_seq_len, 256) * kv->nkv * B * std::max(1, pl.splits) < (1l << 31) && (long)q_len * p.G * p.G < (1l << 32),
                     "paged_attn_scored: %d rows of %d heads in %d sequences of %d slots exceed the grid", rows, nh, B, max_seq_len);
     int crc;
 #define LB_(HD_) do { if (bf) crc = int8 ? launch_chunk<HD_, true, true>(c, pl, st) : launch_chunk<HD_, false, true>(c, pl, st); \

@@ -739,42 +739,46 @@ def paged_decode_attention(q: torch.Tensor, kv_base: torch.Tensor, scale_base: O
 
 
 # ------------------------------------------------------------------ a cache whose slots are not positions
-def _here(t: torch.Tensor, name: str):
-    """Launches go to the current device's current stream: tensors of another device are refused."""
-    if not t.is_cuda:
+def _on(t: torch.Tensor, name: str) -> int:
+    """The device of a call: launches go to the current device's current stream, tensors of another one are refused."""
+    dev = t.get_device()
+    if dev < 0:
         raise _C.Mi355Error(f"{name}: tensor must live on the GPU (no CPU path exists)")
-    if t.device.index != torch._C._cuda_getDevice():
+    if dev != torch._C._cuda_getDevice():
         raise _C.Mi355Error(f"{name}: tensor on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return dev
 
 
-def _ints(t: Optional[torch.Tensor], n: int, like: torch.Tensor, name: str):
+def _array(t: Optional[torch.Tensor], dtype: torch.dtype, n: int, dev: int, name: str) -> Optional[int]:
+    """The address of a contiguous array of n entries on the call's device, None for None.  (A step makes dozens of these calls: attributes are asked for once each.)"""
     if t is None:
-        return
-    _chk(t, torch.int32, name)
-    if t.numel() != n or t.device != like.device:
-        raise _C.Mi355Error(f"{name}: {tuple(t.shape)} on {t.device} for {n} entries on {like.device}")
+        return None
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise _C.Mi355Error(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected {n} contiguous {dtype} on cuda:{dev}")
+    return t.data_ptr()
 
 
-def _plane(t: Optional[torch.Tensor], dtype, kv: "_C.KVLayer", like: torch.Tensor, name: str):
-    if t is None:
-        return
-    _chk(t, dtype, name)
-    if t.numel() != kv.num_blocks * kv.nkv * kv.page or t.device != like.device:
-        raise _C.Mi355Error(f"{name}: {tuple(t.shape)} on {t.device} for a plane [{kv.num_blocks}, {kv.nkv}, {kv.page}] on {like.device}")
+def _table(t: torch.Tensor, dev: int, name: str) -> int:
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.get_device() != dev or not t.is_contiguous():
+        raise _C.Mi355Error(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, expected contiguous int32 [sequences, blocks] on cuda:{dev}")
+    return t.data_ptr()
 
 
-def _pool(kv_base: torch.Tensor, scale_base: Optional[torch.Tensor], page: int, nkv: int, hd: int, act, like: torch.Tensor, name: str) -> "_C.KVLayer":
-    """kv_struct of a cache that is checked to be a whole pool of such pages."""
-    if kv_base.dtype not in (torch.int8, torch.float16, torch.bfloat16) or not kv_base.is_contiguous() or kv_base.device != like.device:
-        raise _C.Mi355Error(f"{name}: cache {kv_base.dtype} on {kv_base.device} (contiguous int8, float16 or bfloat16 on {like.device})")
-    if min(page, nkv, hd) < 1 or kv_base.numel() == 0 or kv_base.numel() % (2 * nkv * page * hd):
+def _pool(kv_base: torch.Tensor, scale_base: Optional[torch.Tensor], page: int, nkv: int, hd: int, act: Optional[torch.dtype], dev: int, name: str) -> "_C.KVLayer":
+    """kv_struct of a cache that is checked to be a whole pool of such pages (act None: the type that goes with the cache)."""
+    dt, n = kv_base.dtype, kv_base.numel()
+    act = (torch.bfloat16 if dt is torch.bfloat16 else torch.float16) if act is None else act
+    if kv_base.get_device() != dev or not kv_base.is_contiguous() or (dt is not torch.int8 and dt is not act):
+        raise _C.Mi355Error(f"{name}: cache {dt} {tuple(kv_base.shape)} on {kv_base.device}, expected contiguous int8 or {act} on cuda:{dev}")
+    if page < 1 or nkv < 1 or hd < 1 or n == 0 or n % (2 * nkv * page * hd):
         raise _C.Mi355Error(f"{name}: cache {tuple(kv_base.shape)} is no pool of blocks of 2 x {nkv} heads x {page} tokens x {hd}")
-    kv = kv_struct(kv_base, scale_base, page, nkv, hd, act)
-    if kv_base.dtype == torch.int8:
-        _chk(scale_base, torch.float32, name + ".scale")
-        if scale_base.numel() != kv.num_blocks * 2 * nkv * page or scale_base.device != like.device:
-            raise _C.Mi355Error(f"{name}: scales {tuple(scale_base.shape)} on {scale_base.device} for [{kv.num_blocks}, 2, {nkv}, {page}]")
-    return kv
+    nblk, scales = n // (2 * nkv * page * hd), 0
+    if dt is torch.int8:
+        if scale_base is None:
+            raise _C.Mi355Error(f"{name}: an int8 cache requires the fp32 scale plane")
+        scales = _array(scale_base, torch.float32, nblk * 2 * nkv * page, dev, name + ".scale")
+    return _C.KVLayer(kv_base.data_ptr(), scales, _C.KV_INT8 if dt is torch.int8 else _C.KV_BF16 if dt is torch.bfloat16 else _C.KV_FP16, page, nkv, hd, nblk,
+                      _C.ACT_BF16 if act is torch.bfloat16 else _C.ACT_F16)
 
 
 def rope_kv_write_slots(qkv: torch.Tensor, qkv_bias: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], positions: torch.Tensor, slots: torch.Tensor,
@@ -785,31 +789,22 @@ def rope_kv_write_slots(qkv: torch.Tensor, qkv_bias: Optional[torch.Tensor], cos
     rotated, for models with distance biases) and stored at slot slots[t] of sequence t // q_len, or row_seq[t] (q_len 1); slots[t] < 0 is a padding row.  The planes key_pos (int32)
     and weights (fp32, [num_blocks, nkv, page]; see kvcache.alloc_planes) receive the position and 0.  -> q [T, nh, hd].  Rows with a position, slot, sequence or block id out of range
     are not stored; oob_count (int32 [1]) counts them."""
-    _chk_act(qkv, "rope_kv_write_slots.qkv"); _here(qkv, "rope_kv_write_slots.qkv")
-    if qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd:
-        raise _C.Mi355Error(f"rope_kv_write_slots: qkv {tuple(qkv.shape)} for ({nh} + 2 x {nkv}) heads of {hd}")
-    T = qkv.shape[0]
-    kv = _pool(kv_base, scale_base, page, nkv, hd, qkv.dtype, qkv, "rope_kv_write_slots")
-    _ints(positions, T, qkv, "rope_kv_write_slots.positions"); _ints(slots, T, qkv, "rope_kv_write_slots.slots"); _ints(row_seq, T, qkv, "rope_kv_write_slots.row_seq")
-    _chk(block_table, torch.int32, "rope_kv_write_slots.block_table")
-    _plane(key_pos, torch.int32, kv, qkv, "rope_kv_write_slots.key_pos"); _plane(weights, torch.float32, kv, qkv, "rope_kv_write_slots.weights")
-    _ints(oob_count, 1, qkv, "rope_kv_write_slots.oob_count")
-    if block_table.dim() != 2 or block_table.device != qkv.device:
-        raise _C.Mi355Error(f"rope_kv_write_slots: block_table {tuple(block_table.shape)} on {block_table.device}")
-    if qkv_bias is not None:
-        _chk(qkv_bias, qkv.dtype, "rope_kv_write_slots.qkv_bias")
-        if qkv_bias.numel() != qkv.shape[1] or qkv_bias.device != qkv.device:
-            raise _C.Mi355Error(f"rope_kv_write_slots: bias {tuple(qkv_bias.shape)} for {qkv.shape[1]} columns")
-    if cos_sin is not None:
-        _chk(cos_sin, torch.float32, "rope_kv_write_slots.cos_sin")
-        if cos_sin.dim() < 2 or cos_sin.shape[0] < 1 or cos_sin.numel() != cos_sin.shape[0] * hd or cos_sin.device != qkv.device:
-            raise _C.Mi355Error(f"rope_kv_write_slots: cos_sin {tuple(cos_sin.shape)} for [positions, {hd // 2}, 2]")
-    q_out = torch.empty(T, nh, hd, dtype=qkv.dtype, device=qkv.device)
-    if T == 0:
-        return q_out
-    _C.check(_C.lib().mi355_rope_kv_write_slots(qkv.data_ptr(), qkv.shape[1], _p(qkv_bias), _p(cos_sin), 0 if cos_sin is None else cos_sin.shape[0], positions.data_ptr(), slots.data_ptr(),
-                                                _p(row_seq), block_table.data_ptr(), block_table.shape[1], block_table.shape[0], T, q_len, nh, C.byref(kv), q_out.data_ptr(),
-                                                _p(key_pos), _p(weights), _p(oob_count), _stream()), "rope_kv_write_slots")
+    w = "rope_kv_write_slots"
+    if qkv.dtype not in ACT_DTYPES or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd or not qkv.is_contiguous():
+        raise _C.Mi355Error(f"{w}: qkv {qkv.dtype} {tuple(qkv.shape)} for contiguous rows of ({nh} + 2 x {nkv}) heads of {hd} in float16 or bfloat16")
+    dev, (T, width) = _on(qkv, w + ".qkv"), qkv.shape
+    kv = _pool(kv_base, scale_base, page, nkv, hd, qkv.dtype, dev, w)
+    i32, plane = torch.int32, kv.num_blocks * nkv * page
+    most = 0 if cos_sin is None else cos_sin.shape[0]
+    if cos_sin is not None and (cos_sin.dim() < 2 or most < 1):
+        raise _C.Mi355Error(f"{w}: cos_sin {tuple(cos_sin.shape)} for [positions, {hd // 2}, 2]")
+    args = (qkv.data_ptr(), width, _array(qkv_bias, qkv.dtype, width, dev, w + ".qkv_bias"), _array(cos_sin, torch.float32, most * hd, dev, w + ".cos_sin"), most,
+            _array(positions, i32, T, dev, w + ".positions"), _array(slots, i32, T, dev, w + ".slots"), _array(row_seq, i32, T, dev, w + ".row_seq"),
+            _table(block_table, dev, w + ".block_table"), block_table.shape[1], block_table.shape[0], T, q_len, nh, C.byref(kv))
+    planes = (_array(key_pos, i32, plane, dev, w + ".key_pos"), _array(weights, torch.float32, plane, dev, w + ".weights"), _array(oob_count, i32, 1, dev, w + ".oob_count"))
+    q_out = qkv.new_empty(T, nh, hd)
+    if T:
+        _C.check(_C.lib().mi355_rope_kv_write_slots(*args, q_out.data_ptr(), *planes, _stream()), w)
     return q_out
 
 
@@ -817,48 +812,38 @@ def paged_attention_scored(q: torch.Tensor, kv_base: torch.Tensor, scale_base: O
                            max_seq_len: int, *, begin: Optional[torch.Tensor] = None, row_start: Optional[torch.Tensor] = None, q_len: int = 1, scale: Optional[float] = None,
                            softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, key_pos: Optional[torch.Tensor] = None,
                            weights: Optional[torch.Tensor] = None, decay: float = 1.0, return_lse: bool = False, out: Optional[torch.Tensor] = None):
-    """q [rows, nh, hd] over a paged cache, rows of sequence b: row_start[b] .. row_start[b + 1] - 1 (int32 [B + 1] on the device, at most q_len each; rows behind the last are left alone), or
-    q_len each without row_start.  A row sees the slots begin[row] .. end[row] - 1 of its sequence (int32; begin None: from 0): causal end = slot + 1, a window begin = end - window, a
-    prefix that all rows see end = max(slot + 1, prefix), packed documents begin = first slot of the row's document; a row that sees nothing gets zeros.
+    """q [rows, nh, hd] over a paged cache (pages of whole 16 tokens), rows of sequence b: row_start[b] .. row_start[b + 1] - 1 (int32 [B + 1] on the device, at most q_len each; rows behind
+    the last are left alone), or q_len each without row_start.  A row sees the slots begin[row] .. end[row] - 1 of its sequence (int32; begin None: from 0): causal end = slot + 1, a window
+    begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = first slot of the row's document; a row that sees nothing gets zeros.
     Scores: softcap * tanh(scale q.k / softcap) for softcap > 0, plus slopes[h] * (key position - positions[row]) with slopes (fp32 [nh]), key positions from the plane key_pos
     (int32 [num_blocks, nkv, page]) or the slots themselves.
     weights (fp32 plane) <- decay * weights + the probabilities of the call's rows and of the heads of each kv head, for the slots below the largest end
     of each sequence's rows that see something; kv_evict ranks by it.
     The rows of q may have any stride of whole 16-byte pieces.  -> out [rows, nh * hd], with return_lse (out, log-sum-exp fp32 [rows, nh], -inf for a row that sees nothing)."""
+    w = "paged_attention_scored"
     if q.dtype not in ACT_DTYPES or q.dim() != 3:
-        raise _C.Mi355Error(f"paged_attention_scored: q {q.dtype} {tuple(q.shape)} (float16 or bfloat16, [rows, heads, channels])")
-    _here(q, "paged_attention_scored.q")
-    T, nh, hd = q.shape
-    if q.stride(2) != 1 or q.stride(1) != hd or (T > 1 and q.stride(0) < nh * hd):
-        raise _C.Mi355Error(f"paged_attention_scored: strides {q.stride()} of q {tuple(q.shape)} (heads of a row side by side)")
-    kv = _pool(kv_base, scale_base, page, nkv, hd, q.dtype, q, "paged_attention_scored")
-    _chk(block_table, torch.int32, "paged_attention_scored.block_table")
-    if block_table.dim() != 2 or block_table.device != q.device:
-        raise _C.Mi355Error(f"paged_attention_scored: block_table {tuple(block_table.shape)} on {block_table.device}")
-    B = block_table.shape[0]
-    _ints(end, T, q, "paged_attention_scored.end"); _ints(begin, T, q, "paged_attention_scored.begin"); _ints(positions, T, q, "paged_attention_scored.positions")
-    _ints(row_start, B + 1, q, "paged_attention_scored.row_start")
-    _plane(key_pos, torch.int32, kv, q, "paged_attention_scored.key_pos"); _plane(weights, torch.float32, kv, q, "paged_attention_scored.weights")
-    if slopes is not None:
-        _chk(slopes, torch.float32, "paged_attention_scored.slopes")
-        if slopes.numel() != nh or slopes.device != q.device:
-            raise _C.Mi355Error(f"paged_attention_scored: {tuple(slopes.shape)} slopes for {nh} heads")
+        raise _C.Mi355Error(f"{w}: q {q.dtype} {tuple(q.shape)} (float16 or bfloat16, [rows, heads, channels])")
+    dev, (T, nh, hd), (ld, sh, sd) = _on(q, w + ".q"), q.shape, q.stride()
+    if sd != 1 or sh != hd or (T > 1 and ld < nh * hd):
+        raise _C.Mi355Error(f"{w}: strides {q.stride()} of q {tuple(q.shape)} (heads of a row side by side)")
     if key_pos is not None and slopes is None:
-        raise _C.Mi355Error("paged_attention_scored: key_pos goes with slopes")
+        raise _C.Mi355Error(f"{w}: key_pos goes with slopes")
+    kv = _pool(kv_base, scale_base, page, nkv, hd, q.dtype, dev, w)
+    i32, plane, table = torch.int32, kv.num_blocks * nkv * page, _table(block_table, dev, w + ".block_table")
+    B, M = block_table.shape
+    starts, tracked = _array(row_start, i32, B + 1, dev, w + ".row_start"), _array(weights, torch.float32, plane, dev, w + ".weights")
+    sc = _C.AttnScore(hd ** -0.5 if scale is None else scale, softcap, _array(slopes, torch.float32, nh, dev, w + ".slopes"), _array(positions, i32, T, dev, w + ".positions"),
+                      _array(key_pos, i32, plane, dev, w + ".key_pos"), _array(begin, i32, T, dev, w + ".begin"), _array(end, i32, T, dev, w + ".end"))
     if out is None:
-        out = torch.empty(T, nh * hd, dtype=q.dtype, device=q.device)
-    else:
-        _chk(out, q.dtype, "paged_attention_scored.out")
-        if out.numel() != T * nh * hd or out.device != q.device:
-            raise _C.Mi355Error(f"paged_attention_scored: out {tuple(out.shape)} for [{T}, {nh * hd}]")
+        out = q.new_empty(T, nh * hd)
+    to = _array(out, q.dtype, T * nh * hd, dev, w + ".out")
     lse = torch.empty(T, nh, dtype=torch.float32, device=q.device) if return_lse else None
     if T and B:
         l = _C.lib()
-        need = l.mi355_paged_attn_scored_workspace_bytes(B, q_len, T, nh, nkv, hd, max_seq_len, int(weights is not None))
+        need = l.mi355_paged_attn_scored_workspace_bytes(B, q_len, T, nh, nkv, hd, max_seq_len, int(tracked is not None))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None       # of this call alone: calls on other streams or in graphs have their own
-        sc = _C.AttnScore(hd ** -0.5 if scale is None else scale, softcap, _p(slopes), _p(positions), _p(key_pos), _p(begin), end.data_ptr())
-        _C.check(l.mi355_paged_attn_scored(q.data_ptr(), q.stride(0) if T > 1 else nh * hd, C.byref(kv), block_table.data_ptr(), block_table.shape[1], _p(row_start), B, q_len, T, nh,
-                                           C.byref(sc), max_seq_len, out.data_ptr(), _p(lse), _p(weights), decay, _p(ws), need, _stream()), "paged_attn_scored")
+        _C.check(l.mi355_paged_attn_scored(q.data_ptr(), ld if T > 1 else nh * hd, C.byref(kv), table, M, starts, B, q_len, T, nh, C.byref(sc), max_seq_len, to, _p(lse), tracked, decay,
+                                           _p(ws), need, _stream()), w)
     return (out, lse) if return_lse else out
 
 
@@ -868,22 +853,19 @@ def kv_evict(weights: torch.Tensor, key_pos: torch.Tensor, block_table: torch.Te
     (sinks + recent <= keep), the others by their weight, the lower slot first where weights are equal.  Survivors behind slot keep - 1 move into the slots below that became free, with their
     scales, weights and positions; what the slots from `keep` on hold afterwards is unspecified.  weights, key_pos: planes [num_blocks, nkv, page]; kv_base [num_blocks, 2, nkv,
     page, hd]; seq_lens, next_pos int32 [B] on the device; the pages of block_table are each sequence's own.  -> the new lengths (int32 [B]); the next token goes to that slot."""
-    if weights.dim() != 3 or kv_base.dim() != 5:
-        raise _C.Mi355Error(f"kv_evict: weights {tuple(weights.shape)}, cache {tuple(kv_base.shape)} (planes [blocks, heads, page] of a cache [blocks, 2, heads, page, channels])")
-    _here(kv_base, "kv_evict.kv_base")
-    _, nkv, page = weights.shape
-    kv = _pool(kv_base, scale_base, page, nkv, kv_base.shape[4], None, kv_base, "kv_evict")
-    _plane(weights, torch.float32, kv, kv_base, "kv_evict.weights"); _plane(key_pos, torch.int32, kv, kv_base, "kv_evict.key_pos")
-    _chk(block_table, torch.int32, "kv_evict.block_table")
-    if block_table.dim() != 2 or block_table.device != kv_base.device or kv_base.shape[2] != nkv or kv_base.shape[3] != page:
-        raise _C.Mi355Error(f"kv_evict: block_table {tuple(block_table.shape)} on {block_table.device}, cache {tuple(kv_base.shape)} against planes {tuple(weights.shape)}")
+    w = "kv_evict"
+    if weights.dim() != 3 or kv_base.dim() != 5 or kv_base.shape[2:4] != weights.shape[1:]:
+        raise _C.Mi355Error(f"{w}: weights {tuple(weights.shape)}, cache {tuple(kv_base.shape)} (planes [blocks, heads, page] of a cache [blocks, 2, heads, page, channels])")
+    dev, (_, nkv, page) = _on(kv_base, w + ".kv_base"), weights.shape
+    kv = _pool(kv_base, scale_base, page, nkv, kv_base.shape[4], None, dev, w)
+    plane, table = kv.num_blocks * nkv * page, _table(block_table, dev, w + ".block_table")
     B, M = block_table.shape
-    _ints(seq_lens, B, kv_base, "kv_evict.seq_lens"); _ints(next_pos, B, kv_base, "kv_evict.next_pos")
+    args = (C.byref(kv), _array(weights, torch.float32, plane, dev, w + ".weights"), _array(key_pos, torch.int32, plane, dev, w + ".key_pos"), table, M,
+            _array(seq_lens, torch.int32, B, dev, w + ".seq_lens"), _array(next_pos, torch.int32, B, dev, w + ".next_pos"))
     new_lens = torch.empty(B, dtype=torch.int32, device=kv_base.device)
     if B:
         l, most = _C.lib(), M * page if max_seq_len is None else max_seq_len
         need = l.mi355_kv_evict_workspace_bytes(B, nkv, keep, most)
         ws = torch.empty(need, dtype=torch.uint8, device=kv_base.device)
-        _C.check(l.mi355_kv_evict(C.byref(kv), weights.data_ptr(), key_pos.data_ptr(), block_table.data_ptr(), M, seq_lens.data_ptr(), next_pos.data_ptr(), B, most, keep, sinks, recent,
-                                  new_lens.data_ptr(), ws.data_ptr(), need, _stream()), "kv_evict")
+        _C.check(l.mi355_kv_evict(*args, B, most, keep, sinks, recent, new_lens.data_ptr(), ws.data_ptr(), need, _stream()), w)
     return new_lens
