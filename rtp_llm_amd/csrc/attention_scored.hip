@@ -23,7 +23,7 @@ namespace {
 // A wave walks its groups on its own.  They come by DMA into a ring of its own in LDS: what is in flight takes no registers, and a page's 16 tokens are one scalar base for loads
 // whose lanes' offsets never change.  A key's 16-byte pieces are swizzled by the token, a channel's 16 values stay side by side.
 //
-// Work: the tokens that any row of a sequence sees, in units of 128 (a group for each of a block's four waves), times key/value heads, laid end to end over all sequences and dealt to the
+// Work: the tokens that any row of a sequence sees, in units of a group of 32 for each of a block's waves, times key/value heads, laid end to end over all sequences and dealt to the
 // blocks in equal runs.  A pair of a sequence and a head that lies inside one run is finished there, others leave a part in each run and scored_join_kernel merges them.  Sequences
 // of unequal length so take the time of their mean: a run may end one pair and begin the next.
 struct DecodeParams : ScoredParams {
@@ -34,7 +34,6 @@ struct DecodeParams : ScoredParams {
     int4*    meta;       // [pairs]: first slot, parts, the sequence's first seen slot rounded down to 32, its reach
     int      nblocks, ncol, ctx_pad, runs;   // runs: 0 = a block per pair
 };
-constexpr int UNIT = 128;
 
 // The slots that a sequence's rows see, [seen, hi), and lo = seen down to 32; nothing: zeros.
 __device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int len, int& lo, int& hi, int& seen) {
@@ -47,7 +46,6 @@ __device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int
     if (hi == 0) seen = 0;
     lo = seen & ~31;
 }
-__device__ __forceinline__ int units_of(int lo, int hi) { return (hi - lo + UNIT - 1) / UNIT; }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -68,26 +66,31 @@ template <bool BF> __device__ __forceinline__ u32x4 widen_codes(uint32_t lo, uin
     return v;
 }
 
-// LDS of a wave's stage: keys, values, and (EXTRA) 1 KB of scales and positions; stages that 160 KB hold, as many as pay.
-template <int HD, bool INT8, bool EXTRA> struct Ring {
-    static constexpr int ES = INT8 ? 1 : 2, KB = 32 * HD * ES, LOADS = 2 * KB / 1024 + (EXTRA ? 1 : 0), STAGE = LOADS * 1024, N = HD == 128 && !INT8 ? 2 : INT8 && HD == 128 ? 4 : 4;
-    static constexpr int MERGE = 4 * 16 * (HD + 4) * 4 + 2 * 4 * 16 * 4, BYTES = 4 * N * STAGE > MERGE ? 4 * N * STAGE : MERGE;
+// Waves of a block, LDS of a wave's stage (keys, values, and, EXTRA, 1 KB of scales and positions), stages.  What is in flight fills LDS either way; eight waves, two a SIMD, hide what a group's chain
+// of product, softmax and product leaves idle, where a stage is 8 KB or less and the registers of two tiles of columns are not in the way.
+template <int HD, bool INT8, int NT, bool EXTRA> struct Ring {
+    static constexpr int ES = INT8 ? 1 : 2, KB = 32 * HD * ES, LOADS = 2 * KB / 1024 + (EXTRA ? 1 : 0), STAGE = LOADS * 1024, NW = NT == 1 && (INT8 || HD == 64) ? 8 : 4;
+    static constexpr int N = HD == 128 && !INT8 ? 2 : NW == 4 ? 4 : HD == 64 && INT8 ? 3 : 2, UNIT = 32 * NW;
+    static constexpr int MERGE = NW * 16 * (HD + 4) * 4 + 2 * NW * 16 * 4, BYTES = NW * N * STAGE > MERGE ? NW * N * STAGE : MERGE;
+    static_assert(BYTES <= 160 * 1024 && LOADS * (N - 1) < 63, "");
 };
 
 template <int HD, bool INT8, int NT, bool BF, bool KP>
-__global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p) {
+__global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void scored_decode_kernel(const DecodeParams p) {
     constexpr bool EXTRA = INT8 || KP;
     // 8 bits under fp16: probabilities take the value's scale, an amax / 127, before they are rounded.  64 of it keep the small ones out of fp16's subnormals (amax <= 65504: 64 scales fit) if
     // no probability exceeds 1.
     constexpr float VS = INT8 && !BF ? 64.f : 1.f, DEFER = INT8 && !BF ? 0.f : 6.f;
-    using R = Ring<HD, INT8, EXTRA>;
+    using R = Ring<HD, INT8, NT, EXTRA>;
+    constexpr int NW = R::NW, UNIT = R::UNIT, NTHR = 64 * NW;
+    auto units_of = [](int from, int to) { return (to - from + UNIT - 1) / UNIT; };
     constexpr int NSTEP = HD / 32, NDB = HD / 16, ES = R::ES, CK = HD * ES / 16, RS = R::N;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int j = lane & 15, w = lane >> 4;
     extern __shared__ __attribute__((aligned(16))) char dec_sm[];
     auto s_o = reinterpret_cast<float(*)[16][HD + 4]>(dec_sm);                        // the merge's, over the ring
-    auto s_m = reinterpret_cast<float(*)[16]>(dec_sm + 4 * 16 * (HD + 4) * 4);
-    float(*s_l)[16] = s_m + 4;
+    auto s_m = reinterpret_cast<float(*)[16]>(dec_sm + NW * 16 * (HD + 4) * 4);
+    float(*s_l)[16] = s_m + NW;
     char* ring = dec_sm + wave * RS * R::STAGE;
     const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
     // lanes' offsets in loads of keys (R::KB / 1024 of them, 1024 / (HD ES) rows each) and values
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
             wait_vm<63>();                          // the stage has been read before a later load may land in it
         }
         __syncthreads();                            // every wave is done with its ring
-        // ---- the four waves meet in LDS, a tile of columns at a time
+        // ---- the waves meet in LDS, a tile of columns at a time
         const size_t slot = (size_t)blockIdx.x * 2 + (first ? 0 : 1);
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -388,13 +391,15 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
             if (w == 0) { s_m[wave][j] = m_run[c]; s_l[wave][j] = lr; }
             __syncthreads();
             const int here = min(16, ncol - c * 16);
-            for (int idx = tid; idx < here * (HD / 4); idx += 256) {
+            for (int idx = tid; idx < here * (HD / 4); idx += NTHR) {
                 const int jj = idx / (HD / 4), d0 = (idx - jj * (HD / 4)) * 4, col = c * 16 + jj;
-                const float mstar = fmaxf(fmaxf(s_m[0][jj], s_m[1][jj]), fmaxf(s_m[2][jj], s_m[3][jj]));
+                float mstar = s_m[0][jj];
+#pragma unroll
+                for (int ww = 1; ww < NW; ++ww) mstar = fmaxf(mstar, s_m[ww][jj]);
                 f32x4 acc = {0.f, 0.f, 0.f, 0.f};
                 float l = 0.f;
 #pragma unroll
-                for (int ww = 0; ww < 4; ++ww) {
+                for (int ww = 0; ww < NW; ++ww) {
                     const float f = __builtin_amdgcn_exp2f(s_m[ww][jj] - mstar);
                     const f32x4 ow = *reinterpret_cast<const f32x4*>(&s_o[ww][jj][d0]);
                     acc += ow * f;
@@ -428,76 +433,98 @@ __global__ __launch_bounds__(256) void scored_decode_kernel(const DecodeParams p
     }
 }
 
-// What the runs left: a wave per (pair, column) merges its parts (nothing to do where there is one; zeros where there is none), and, behind those blocks, a thread per slot adds the
+// What the runs left: columns whose pair has several parts are merged (zeros where there is none), and, behind those blocks, a thread per slot adds the
 // probabilities of all columns to the slot's weight.
-template <int HD, bool BF>
+template <int HD, bool BF, int SL, int CPB>
 __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, int join_blocks, int chunks) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     auto slot_of = [](const int4& mt, int i) { return i == 0 ? mt.x : (mt.x / 2 + i) * 2; };
     if ((int)blockIdx.x < join_blocks) {
-        const int gid = blockIdx.x * 4 + wave, pair = gid / p.ncol, col = gid - pair * p.ncol;
-        if (pair >= p.B * p.nkv) return;
+        // CPB columns a block; groups of HD / 4 threads share a column's parts, eight in flight each: few columns, whose pairs have many parts, take a block each (heads of 128: 64 parts in one
+        // round trip), many take a wave
+        constexpr int TP = HD / 4, NG = 256 / TP, NGC = NG / CPB;
+        __shared__ f32x4 s_acc[NG][TP];
+        __shared__ float2 s_ml[NG];
+        const int all_grp = tid / TP, grp = all_grp % NGC, d0 = tid % TP * 4, gid = blockIdx.x * CPB + all_grp / NGC;
+        const int pair = min(gid / p.ncol, p.B * p.nkv - 1), col = gid % p.ncol, b = pair / p.nkv, kh = pair - b * p.nkv;
         const int4 mt = p.meta[pair];
-        if (mt.y == 1) return;
-        const int b = pair / p.nkv, kh = pair - b * p.nkv;
         int base, len;
         scored_rows_of(p, b, base, len);
-        if (col >= len * p.G) return;
-        const int rl = col / p.G, row = base + rl, h = kh * p.G + (col - rl * p.G);
-        float m = NEG_BIG;
-        for (int i = lane; i < mt.y; i += 64) m = fmaxf(m, p.tmp_ml[((size_t)slot_of(mt, i) * p.ncol + col) * 2]);
-        m = wave_max(m);
-        constexpr int CPL = HD / 64;
-        float l = 0.f, acc[CPL];
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
-        for (int i0 = 0; i0 < mt.y; i0 += 8) {      // eight parts in flight, added in their order
+        const bool on = gid < p.B * p.nkv * p.ncol && mt.y != 1 && col < len * p.G;
+        const int rl = on ? col / p.G : 0, row = on ? base + rl : 0, h = kh * p.G + (on ? col - rl * p.G : 0);
+        float m = NEG_BIG, l = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = grp; on && i0 < mt.y; i0 += NGC * 8) {
             float2 ml[8];
-            float v[8][CPL];
+            f32x4 v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const size_t at = (size_t)slot_of(mt, min(i0 + i, mt.y - 1)) * p.ncol + col;
+                const size_t at = (size_t)slot_of(mt, min(i0 + i * NGC, mt.y - 1)) * p.ncol + col;
                 ml[i] = *reinterpret_cast<const float2*>(p.tmp_ml + at * 2);
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) v[i][c] = p.tmp_out[at * HD + lane * CPL + c];
+                v[i] = *reinterpret_cast<const f32x4*>(p.tmp_out + at * HD + d0);
             }
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+            const float f0 = __builtin_amdgcn_exp2f(m - mn);
+            l *= f0; acc *= f0; m = mn;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (i0 + i >= mt.y) continue;
+                if (i0 + i * NGC >= mt.y) continue;
                 const float f = __builtin_amdgcn_exp2f(ml[i].x - m);
                 l += ml[i].y * f;
-#pragma unroll
-                for (int c = 0; c < CPL; ++c) acc[c] += v[i][c] * f;
+                acc += v[i] * f;
             }
+        }
+        s_acc[all_grp][tid % TP] = acc;
+        if (d0 == 0) s_ml[all_grp] = make_float2(m, l);
+        __syncthreads();
+        if (grp != 0 || !on) return;
+        float mn = m;
+#pragma unroll
+        for (int g = 1; g < NGC; ++g) mn = fmaxf(mn, s_ml[all_grp + g].x);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn);
+        l *= f0; acc *= f0;
+#pragma unroll
+        for (int g = 1; g < NGC; ++g) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[all_grp + g].x - mn);
+            l += s_ml[all_grp + g].y * f;
+            acc += s_acc[all_grp + g][tid % TP] * f;
         }
         int a, e;
         scored_interval(p, row, a, e);
-        const float inv = scored_inv(l, e > a);
-        uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((size_t)row * p.nh + h) * HD + lane * CPL;
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) dst[c] = act_to_bits<BF>(acc[c] * inv);
-        if (lane == 0 && p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, e > a, p.slopes && e > a ? scored_shift(p, row, h, scored_ref(p, b, kh, mt.w)) : 0.f);
+        scored_store<BF>(p, row, h, HD, d0, acc, mn, l, e > a, p.slopes && e > a ? scored_ref(p, b, kh, mt.w) : 0);
         return;
     }
-    // ---- weights
+    // ---- weights: SL slots a thread, the first scores asked for before the columns' maxima and sums are merged
     __shared__ float s_m[32], s_i[32];
+    typedef float slots __attribute__((ext_vector_type(SL)));
     const int id = blockIdx.x - join_blocks, pair = id / chunks, chunk = id - pair * chunks;
     const int4 mt = p.meta[pair];
-    if (chunk * 1024 >= mt.w) return;
+    if (chunk * 256 * SL >= mt.w) return;
     const int b = pair / p.nkv, kh = pair - b * p.nkv;
     int base, len;
     scored_rows_of(p, b, base, len);
     const int ncol = len * p.G;
+    const int t = (chunk * 256 + tid) * SL;                          // four slots lie inside a page
+    const bool in = t < mt.w;
+    const int blk = in ? p.block_table[(size_t)b * p.max_blocks + (int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)] : -1;
+    const float* sp = p.spill + (size_t)pair * p.ncol * p.ctx_pad + max(t - mt.z, 0);
+    const bool some = in && t >= mt.z;
+    slots v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (some) v[i] = *reinterpret_cast<const slots*>(sp + (size_t)min(i, ncol - 1) * p.ctx_pad);
     for (int col = wave; col < ncol; col += 4) {
         float m = NEG_BIG, l = 0.f;
         if (mt.y == 1) {
-            const float2 v = *reinterpret_cast<const float2*>(p.ml_all + ((size_t)pair * p.ncol + col) * 2);
-            m = v.x; l = v.y;
+            const float2 x = *reinterpret_cast<const float2*>(p.ml_all + ((size_t)pair * p.ncol + col) * 2);
+            m = x.x; l = x.y;
         } else {
             for (int i = lane; i < mt.y; i += 64) {
-                const float2 v = *reinterpret_cast<const float2*>(p.tmp_ml + ((size_t)slot_of(mt, i) * p.ncol + col) * 2);
-                const float mn = fmaxf(m, v.x);
-                l = l * __builtin_amdgcn_exp2f(m - mn) + v.y * __builtin_amdgcn_exp2f(v.x - mn);
+                const float2 x = *reinterpret_cast<const float2*>(p.tmp_ml + ((size_t)slot_of(mt, i) * p.ncol + col) * 2);
+                const float mn = fmaxf(m, x.x);
+                l = l * __builtin_amdgcn_exp2f(m - mn) + x.y * __builtin_amdgcn_exp2f(x.x - mn);
                 m = mn;
             }
             const float mine = m;
@@ -509,33 +536,28 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
         if (lane == 0) { s_m[col] = m; s_i[col] = scored_inv(l, e > a); }
     }
     __syncthreads();
-    const int t = chunk * 1024 + tid * 4;           // four slots: inside a page (a multiple of 8 tokens)
-    if (t >= mt.w) return;
-    const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
-    const int blk = bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)];
-    if (blk < 0 || blk >= p.num_blocks) return;
+    if (!in || blk < 0 || blk >= p.num_blocks) return;
     float* to = p.weights + ((size_t)blk * p.nkv + kh) * p.page + t % p.page;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (t >= mt.z) {
-        const float* sp = p.spill + (size_t)pair * p.ncol * p.ctx_pad + (t - mt.z);
-        for (int c0 = 0; c0 < ncol; c0 += 8) {
-            f32x4 v[8];
+    slots old, sum;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const f32x4*>(sp + (size_t)min(c0 + i, ncol - 1) * p.ctx_pad);
+    for (int e = 0; e < SL; ++e) { sum[e] = 0.f; old[e] = t + e < mt.w ? to[e] : 0.f; }
+    if (some)
+        for (int c0 = 0; c0 < ncol; c0 += 8) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (c0 + i >= ncol) continue;
                 const float m = s_m[c0 + i], inv = s_i[c0 + i];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += v[i][e] <= NEG_BIG || inv == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[i][e] - m) * inv;
+                for (int e = 0; e < SL; ++e) sum[e] += v[i][e] <= NEG_BIG || inv == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[i][e] - m) * inv;
+            }
+            if (c0 + 8 < ncol) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const slots*>(sp + (size_t)min(c0 + 8 + i, ncol - 1) * p.ctx_pad);
             }
         }
-    }
-    if (t + 4 <= mt.w) {
-        const f32x4 old = *reinterpret_cast<const f32x4*>(to);
-        *reinterpret_cast<f32x4*>(to) = f32x4{scored_decayed(p, old[0], sum[0]), scored_decayed(p, old[1], sum[1]), scored_decayed(p, old[2], sum[2]), scored_decayed(p, old[3], sum[3])};
-    } else
-        for (int e = 0; t + e < mt.w; ++e) to[e] = scored_decayed(p, to[e], sum[e]);
+#pragma unroll
+    for (int e = 0; e < SL; ++e)
+        if (t + e < mt.w) to[e] = scored_decayed(p, old[e], sum[e]);
 }
 
 // ================================================================================================ many rows
@@ -1138,7 +1160,7 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         const long pairs = (long)B * nkv;
         pl.runs = pairs < 4 * RUNS;                              // beyond, pairs are many enough to even out by themselves, and nothing has to be merged
         pl.nblocks = pl.runs ? RUNS : (int)pairs;
-        pl.ncol = q_len * G; pl.ctx_pad = (max_seq + 31 + UNIT) / 32 * 32;
+        pl.ncol = q_len * G; pl.ctx_pad = (max_seq + 63) / 32 * 32 + 32;
         pl.meta = region(pairs * sizeof(int4));
         if (pl.runs) { pl.tmp_out = region((size_t)2 * RUNS * pl.ncol * hd * 4); pl.tmp_ml = region((size_t)2 * RUNS * pl.ncol * 8); }
         if (track) { pl.ml_all = region(pairs * pl.ncol * 8); pl.spill = region(pairs * pl.ncol * pl.ctx_pad * 4); }
@@ -1167,10 +1189,10 @@ template <int HD, bool INT8, int NT, bool BF>
 int launch_decode(const DecodeParams& d, hipStream_t st) {
     auto run = [&](auto kernel, int lds) -> int {
         const int rc = raise_dynamic_lds((const void*)kernel, "paged_attn_scored");
-        if (rc == MI355_OK) hipLaunchKernelGGL(kernel, dim3(d.nblocks), dim3(256), lds, st, d);
+        if (rc == MI355_OK) hipLaunchKernelGGL(kernel, dim3(d.nblocks), dim3(64 * Ring<HD, INT8, NT, true>::NW), lds, st, d);
         return rc;
     };
-    return d.key_pos ? run(scored_decode_kernel<HD, INT8, NT, BF, true>, Ring<HD, INT8, true>::BYTES) : run(scored_decode_kernel<HD, INT8, NT, BF, false>, Ring<HD, INT8, INT8>::BYTES);
+    return d.key_pos ? run(scored_decode_kernel<HD, INT8, NT, BF, true>, Ring<HD, INT8, NT, true>::BYTES) : run(scored_decode_kernel<HD, INT8, NT, BF, false>, Ring<HD, INT8, NT, INT8>::BYTES);
 }
 
 template <int HD, bool INT8, bool BF, int FORM>
@@ -1234,10 +1256,17 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
 #undef LN_
         if (lrc != MI355_OK) return lrc;
         MI355_CHECK_LAUNCH("scored_decode_kernel");
-        const int pairs = B * kv->nkv, chunks = weights ? cdiv(max_seq_len, 1024) : 0, joins = cdiv(pairs * pl.ncol, 4);
+        // four slots a thread, or one where that leaves less than two blocks a compute unit
+        const int pairs = B * kv->nkv, sl = (long)pairs * cdiv(max_seq_len, 1024) >= 512 ? 4 : 1, chunks = weights ? cdiv(max_seq_len, 256 * sl) : 0;
+        const bool wide = pairs < 64;                            // at least four runs a pair
+        const int joins = wide ? pairs * pl.ncol : cdiv(pairs * pl.ncol, 4);
         const dim3 grid(joins + pairs * chunks);
-        if (kv->hd == 128) { if (bf) hipLaunchKernelGGL((scored_join_kernel<128, true>), grid, dim3(256), 0, st, p, joins, chunks); else hipLaunchKernelGGL((scored_join_kernel<128, false>), grid, dim3(256), 0, st, p, joins, chunks); }
-        else               { if (bf) hipLaunchKernelGGL((scored_join_kernel<64, true>), grid, dim3(256), 0, st, p, joins, chunks); else hipLaunchKernelGGL((scored_join_kernel<64, false>), grid, dim3(256), 0, st, p, joins, chunks); }
+#define LK_(HD_, BF_, SL_) do { if (wide) hipLaunchKernelGGL((scored_join_kernel<HD_, BF_, SL_, 1>), grid, dim3(256), 0, st, p, joins, chunks); \
+                                else      hipLaunchKernelGGL((scored_join_kernel<HD_, BF_, SL_, 4>), grid, dim3(256), 0, st, p, joins, chunks); } while (0)
+#define LJ_(HD_, BF_) do { if (sl == 4) LK_(HD_, BF_, 4); else LK_(HD_, BF_, 1); } while (0)
+        if (kv->hd == 128) { if (bf) LJ_(128, true); else LJ_(128, false); } else { if (bf) LJ_(64, true); else LJ_(64, false); }
+#undef LJ_
+#undef LK_
         MI355_CHECK_LAUNCH("scored_join_kernel");
         return MI355_OK;
     }
