@@ -405,8 +405,8 @@ int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias,
  *     u = scale q.k;   s = softcap > 0 ? softcap tanh(u / softcap) : u;   with slopes: s += slopes[h] (key position - positions[row]),
  *   the key position from key_pos, or the slot itself where that is null.  Row r sees the slots begin[r] .. end[r] - 1 of its sequence (begin null: from 0; end is clamped to
  *   max_seq_len): causal rows have end = slot + 1, a window begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = the document's
- *   first slot.  A row that sees nothing gets zeros and a log-sum-exp of -inf.  Block ids are clamped into the pool; what slots that no row of a sequence sees hold, NaN
- *   included, does not matter.
+ *   first slot.  A row that sees nothing gets zeros and a log-sum-exp of -inf.  Block ids are clamped into the pool.  What a slot holds,
+ *   infinities and NaN included, reaches the rows that see it and no others.  scale > 0; softcap 0 (none) or 1e-6 .. 1e6.
  *   Pages of whole 16 tokens.  q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows behind the last are left alone), or, row_start null,
  *   b q_len .. and rows = B q_len.  out [rows][nh hd]; lse [rows][nh] (fp32, natural logarithm) or null.  Any number of heads per kv head.
  *   weights (plane, or null): for every slot below the largest end of its sequence's rows that see something, weights <- decay weights + the sum over the sequence's rows and the heads of the

@@ -16,6 +16,36 @@
 
 namespace {
 
+// Values that are not finite, in slots that some rows see and others do not: the second product would make zero times one, not a number, of them in the rows that do not.  Where a tile is
+// masked its fragments (8 values of 16 bits) are looked at, and from one that has some they go into two of their own, as 2^127 where a row that sees the slot gets +inf (+inf, NaN) and as
+// -2^127 where it gets -inf (-inf, NaN); times 2^127 for a slot that a column sees and 0 for others, in bf16, they become just that, and both together NaN.
+template <bool BF> __device__ __forceinline__ uint32_t odd_bits(u32x4 a) {          // not 0: an exponent of ones
+    constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, ONE = BF ? 0x00800080u : 0x04000400u;
+    return (((a[0] & E) + ONE) | ((a[1] & E) + ONE) | ((a[2] & E) + ONE) | ((a[3] & E) + ONE)) & 0x80008000u;
+}
+template <bool BF> __device__ __forceinline__ void take_odd(u32x4& a, u32x4& up, u32x4& down) {
+    constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u, BIG = 0x7F00u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t keep = 0, u = 0, d = 0;
+#pragma unroll
+        for (int x = 0; x < 32; x += 16) {
+            const uint32_t v = a[w] >> x & 0xFFFFu, mag = v & 0x7FFFu;
+            keep |= mag < E ? v << x : 0u;
+            u |= mag > E || v == E ? BIG << x : 0u;
+            d |= mag > E || (mag == E && v != E) ? (BIG | 0x8000u) << x : 0u;
+        }
+        a[w] = keep; up[w] = u; down[w] = d;
+    }
+}
+// 2^127 in bf16 for those of the 8 slots t .. t + 7 in [lo, hi)
+__device__ __forceinline__ u32x4 seen_big(int t, int lo, int hi) {
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) r[w] = (t + 2 * w >= lo && t + 2 * w < hi ? 0x7F00u : 0u) | (t + 2 * w + 1 >= lo && t + 2 * w + 1 < hi ? 0x7F000000u : 0u);
+    return r;
+}
+
 // ================================================================================================ few rows
 // A (row, head) pair of a sequence's key/value head is one of 16 columns of v_mfma_f32_16x16x32: S^T = K q^T with 16 tokens and O^T = V^T P with 16 channels as rows, so keys and values are
 // read once for up to 32 pairs (two tiles of columns).  The two 16-token halves of a 32-token group take the tokens {8 w + r} and {8 w + 4 + r}, w = lane / 16, so that the lane that holds
@@ -35,16 +65,16 @@ struct DecodeParams : ScoredParams {
     int      nblocks, ncol, ctx_pad, runs;   // runs: 0 = a block per pair
 };
 
-// The slots that a sequence's rows see, [seen, hi), and lo = seen down to 32; nothing: zeros.
-__device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int len, int& lo, int& hi, int& seen) {
-    seen = 0x7fffffff; hi = 0;
+// The slots that a sequence's rows see lie in [lo, hi), lo a multiple of 32; nothing: zeros.
+__device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int len, int& lo, int& hi) {
+    int seen = 0x7fffffff;
+    hi = 0;
     for (int i = 0; i < len; ++i) {
         int a, e;
         scored_interval(p, base + i, a, e);
         if (e > a) { seen = min(seen, a); hi = max(hi, e); }
     }
-    if (hi == 0) seen = 0;
-    lo = seen & ~31;
+    lo = hi == 0 ? 0 : seen & ~31;
 }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -107,15 +137,15 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
     const int ktok = (j & 3) + 8 * (j >> 2), kf = ((j & 3) | (j >> 2) << 2) & (CK - 1);
 
     // ---- this block's run of units.  Lane i looks at sequence i of each 64; up to 64 sequences its answers are all that the block needs of them.
-    int b, kh, lo, hi, seen0, base, len, units, u, u1;  // the pair at hand, its span and rows, the run's next unit inside it, the run's end (counted from the pair's first unit)
-    int my_lo = 0, my_hi = 0, my_seen = 0, my_base = 0, my_len = 0;
+    int b, kh, lo, hi, base, len, units, u, u1;  // the pair at hand, its span and rows, the run's next unit inside it, the run's end (counted from the pair's first unit)
+    int my_lo = 0, my_hi = 0, my_base = 0, my_len = 0;
     auto look = [&](int b0) {
-        my_lo = my_hi = my_seen = my_base = my_len = 0;
-        if (b0 + lane < p.B) { scored_rows_of(p, b0 + lane, my_base, my_len); scored_span(p, my_base, my_len, my_lo, my_hi, my_seen); }
+        my_lo = my_hi = my_base = my_len = 0;
+        if (b0 + lane < p.B) { scored_rows_of(p, b0 + lane, my_base, my_len); scored_span(p, my_base, my_len, my_lo, my_hi); }
     };
     auto take = [&](int who) {
         if (p.B > 64) { look(who & ~63); who &= 63; }
-        lo = __builtin_amdgcn_readlane(my_lo, who); hi = __builtin_amdgcn_readlane(my_hi, who); seen0 = __builtin_amdgcn_readlane(my_seen, who);
+        lo = __builtin_amdgcn_readlane(my_lo, who); hi = __builtin_amdgcn_readlane(my_hi, who);
         base = __builtin_amdgcn_readlane(my_base, who); len = __builtin_amdgcn_readlane(my_len, who);
         units = units_of(lo, hi);
     };
@@ -158,8 +188,8 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
     } else {
         b = blockIdx.x / p.nkv; kh = blockIdx.x - b * p.nkv;
         scored_rows_of(p, b, base, len);
-        scored_span(p, base, len, lo, hi, seen0);
-        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi); seen0 = __builtin_amdgcn_readfirstlane(seen0);
+        scored_span(p, base, len, lo, hi);
+        lo = __builtin_amdgcn_readfirstlane(lo); hi = __builtin_amdgcn_readfirstlane(hi);
         base = __builtin_amdgcn_readfirstlane(base); len = __builtin_amdgcn_readfirstlane(len);
         units = units_of(lo, hi); u = 0; u1 = units;
         if (tid == 0) p.meta[blockIdx.x] = make_int4(0, units ? 1 : 0, lo, hi);
@@ -352,10 +382,15 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
                     a = widen_codes<BF>(v8[0], v8[1]);
                 } else {
                     a = *reinterpret_cast<const u32x4*>(vch);
-                    if (MASKED) {                   // slots that no row sees may hold anything, NaN too: their weights are zero, their values are made so
+                    if (MASKED && __builtin_amdgcn_ballot_w64(odd_bits<BF>(a) != 0)) {
+                        u32x4 up, down;
+                        take_odd<BF>(a, up, down);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (vwin + e >= hi || vwin + e < seen0) a[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+                        for (int c = 0; c < NT; ++c) {
+                            const u32x4 big = seen_big(vwin, c_lo[c], c_hi[c]);
+                            o[c][db] = mfma_act<true>(up, big, o[c][db]);
+                            o[c][db] = mfma_act<true>(down, big, o[c][db]);
+                        }
                     }
                 }
 #pragma unroll
@@ -825,26 +860,44 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             for (int e = 0; e < 8; ++e) {
                 pe[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[k * 8 + e], mul, -m));
                 psum += pe[e];
-                if constexpr (INT8) {
-                    const float vs = (reinterpret_cast<const float*>(st + 2 * KB) + 64)[g * 32 + k * 16 + half * 8 + e] * VS;
-                    pe[e] *= vs;
+            }
+            if constexpr (INT8) {
+                const f32x4* vs = reinterpret_cast<const f32x4*>(st + 2 * KB) + 16 + g * 8 + k * 4 + half * 2;
+                if (masked) {                       // a scale that is not finite is that of the rows that see it
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pe[e] = pe[e] == 0.f ? 0.f : pe[e] * (vs[e >> 2][e & 3] * VS);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pe[e] *= vs[e >> 2][e & 3] * VS;
                 }
             }
             pf[k] = act_pack8<BF>(pe);
         }
         l += psum;
     };
-    auto add = [&](u32x4 (&f)[2][NDB], const u32x4 (&pf)[2], int t0) {
-        if (!INT8 && (t0 + 32 > khi || t0 < seen0)) {        // slots that no row here sees may hold anything, NaN too: their weights are zero, their values are made so
+    auto add = [&](u32x4 (&f)[2][NDB], const u32x4 (&pf)[2], int t0, bool masked) {
+        if (!INT8 && masked) {
+            uint32_t odd = 0;
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int t = t0 + k * 16 + half * 8 + w * 2;
-                    const uint32_t keep = (t < khi && t >= seen0 ? 0xFFFFu : 0u) | (t + 1 < khi && t + 1 >= seen0 ? 0xFFFF0000u : 0u);
+                for (int d = 0; d < NDB; ++d) odd |= odd_bits<BF>(f[k][d]);
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d) f[k][d][w] &= keep;
+                for (int k = 0; k < 2; ++k) {
+                    const u32x4 big = seen_big(t0 + k * 16 + half * 8, lo, hi);
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) {
+                        u32x4 a = f[k][d], up, down;
+                        take_odd<BF>(a, up, down);
+                        // in place, by hand, as the rescaling above, with the waits around both (18 states from a product's issue to a read of its result)
+                        asm volatile("s_nop 15\n\ts_nop 7\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %3, %0\n\ts_nop 15\n\ts_nop 7\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\ts_nop 15\n\ts_nop 7"
+                                     : "+v"(o[d]) : "v"(up), "v"(down), "v"(big));
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) asm volatile("v_mov_b32 %0, %1" : "+v"(f[k][d][w]) : "v"(a[w]));
+                    }
                 }
+            }
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -863,11 +916,11 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
         asm volatile("" ::: "memory");
         weigh(s, st, 0, t0, pf, masked);
         scores(kf1, s);
-        add(vf, pf, t0);
+        add(vf, pf, t0, masked);
         read_values(st, 1, vf);
         asm volatile("" ::: "memory");
         weigh(s, st, 1, t0 + 32, pf, masked);
-        add(vf, pf, t0 + 32);
+        add(vf, pf, t0 + 32, masked);
     };
     if constexpr (!INT8) {
         constexpr int NS = ST::N;
@@ -1064,6 +1117,16 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
             Col c = reinterpret_cast<const Col*>(stage + QB)[cl];
             if (st * 128 + cl >= ncol) c.lo = c.hi = 0;
             if (!__builtin_amdgcn_ballot_w64(c.lo < tw + 64 && c.hi > tw)) continue;
+            if (__builtin_amdgcn_ballot_w64(c.inv != c.inv)) {       // a column that is not a number: so are the slots it sees, and no others
+                const bool odd = c.inv != c.inv;
+                const int a = odd ? c.lo - tw - half * 4 : 0, e = odd ? c.hi - tw - half * 4 : 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {                       // in place, so that the sums are not kept twice
+                    const int t = (i >> 4) * 32 + (i >> 2 & 3) * 8 + (i & 3);
+                    asm volatile("v_add_f32 %0, %0, %1" : "+v"(acc[i >> 4][i & 15]) : "v"(t >= a && t < e ? c.inv : 0.f));
+                }
+                if (odd) { c.lo = c.hi = 0; c.inv = 0.f; }
+            }
             const bool masked = __builtin_amdgcn_ballot_w64(c.lo > tw || c.hi < tw + 64) != 0;
             f32x16 s[2];
 #pragma unroll

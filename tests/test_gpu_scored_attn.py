@@ -147,6 +147,99 @@ def test_row_starts_out_of_range_and_rows_behind_the_last():
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype,int8", [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("nh,nkv,hd,page", [(8, 2, 128, 16), (14, 2, 64, 48)])
+@pytest.mark.parametrize("rows,n", [(3, 90), (70, 150), (300, 300)])
+@pytest.mark.parametrize("what", ["value", "key"])
+def test_what_is_not_finite_reaches_the_rows_that_see_it_alone(nh, nkv, hd, page, dtype, int8, rows, n, what):
+    """Slots that hold infinities or NaN next to slots that others see: a row that sees none of them gets what it gets without them, one that sees them gets the formula's infinities and NaN in
+    their channels (8 bits: a scale that is not a number, NaN in all), and the weights of slots that only untouched rows see stay as they were.
+    Values: bit for bit.  Keys: 64 lanes' columns move their running maxima together, when one of them has grown by enough, so a neighbour's infinite score moves the point from which a
+    column's exponentials are taken.  exp2(s - m) / sum exp2(s - m) does not depend on m, its roundings do: each run is within the formula's bounds, not the same as the other."""
+    g = torch.Generator(device=DEV).manual_seed(rows + hd)
+    kv, sc, bt, dense = make_cache([n], nkv, hd, page, dtype, int8, g, DEV)
+    q = torch.randn(rows, nh, hd, device=DEV, generator=g).to(dtype)
+    r = torch.arange(rows, device=DEV)
+    end = (n - rows + 1 + r).int()
+    begin = torch.where(r % 3 == 0, torch.zeros_like(end), (end - 20).clamp_min(0)).int()
+    begin[1::7] = end[1::7]                                                  # and rows that see nothing
+    bad = {n // 2: float("inf"), n // 2 + 1: float("-inf"), n - 3: float("nan"), n - 30: float("inf")}
+
+    def run():
+        w = torch.full((kv.shape[0], nkv, page), 0.25, device=DEV)
+        out, lse = ops.paged_attention_scored(q, kv, sc, bt, end, nkv, page, bt.shape[1] * page, begin=begin, q_len=rows, weights=w, return_lse=True)
+        return out.view(rows, nh, hd), lse, w
+
+    clean, lse0, w0 = run()
+    for t, x in bad.items():
+        blk, o = int(bt[0, t // page]), t % page
+        if int8:
+            sc[blk, 0 if what == "key" else 1, :, o] = float("nan")
+        elif what == "key":
+            kv[blk, 0, :, o, 5] = x
+        else:
+            kv[blk, 1].view(nkv, hd, page)[:, 5, o] = x
+    out, lse, w = run()
+    sees = {t: (begin <= t) & (t < end) for t in bad}
+    some = torch.stack(list(sees.values())).any(0)
+    assert bool(some.any()) and (rows == 3 or bool((~some & (end > begin)).any()))
+    gw, gw0 = gather_plane(w, bt, 0, n), gather_plane(w0, bt, 0, n)
+    if what == "value":
+        assert torch.equal(out[~some], clean[~some])
+    ref, ref_lse, _, pv, size = attend(q, *dense[0], begin, end, scale=hd ** -0.5)
+    t_out, t_lse, rel = bounds(dtype, hd, n, pv, size, ref)
+    fine = ~some & (end > begin)
+    assert bool(((out.double() - ref).abs() <= t_out)[~some].all())
+    assert bool(((lse.double() - ref_lse).abs() <= t_lse + 2.0 ** -22 * ref_lse.abs())[fine].all()) and bool((lse[end <= begin] == float("-inf")).all())
+    if what == "value":
+        assert torch.equal(lse, lse0) and torch.equal(gw, gw0)               # scores do not look at values
+        if int8:
+            assert bool(torch.isnan(out[some]).all())
+        else:
+            rest = [d for d in range(hd) if d != 5]
+            assert torch.equal(out[:, :, rest], clean[:, :, rest])
+            up, down, nan = (torch.stack([sees[t] for t, x in bad.items() if k(x)]).any(0) for k in (lambda x: x == float("inf"), lambda x: x == float("-inf"), lambda x: x != x))
+            got = out[:, :, 5]
+            assert bool(torch.isnan(got[nan | (up & down)]).all()) and bool((~torch.isfinite(got[some])).all())
+            assert not bool((got[up & ~down & ~nan] == float("-inf")).any()) and not bool((got[down & ~up & ~nan] == float("inf")).any())
+    else:
+        touched = torch.zeros(n, dtype=torch.bool, device=DEV)               # slots that some row sees which sees a bad one too
+        for i in torch.nonzero(some).flatten().tolist():
+            touched[int(begin[i]):int(end[i])] = True
+        t_w = gw0.double() * (2 * float(rel[fine].max() if bool(fine.any()) else 0) + 2.0 ** -21 + rows * (nh // nkv) * 2.0 ** -23)      # two runs of the sums' bounds
+        assert bool(((gw.double() - gw0.double()).abs() <= t_w)[:, ~touched].all())
+        if int8:
+            assert bool(torch.isnan(out[some]).all()) and bool(torch.isnan(gw[:, touched]).all())
+
+
+@pytest.mark.parametrize("dtype,int8", [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)])
+@pytest.mark.parametrize("rows", [2, 4, 40])
+def test_documents_side_by_side_keep_to_themselves(rows, dtype, int8):
+    """Half the rows see [0, 40), half [60, 100): what the first document and the gap between them hold does not reach the second's rows, inside a tile of 32 or across."""
+    nh, nkv, hd, page, n = 8, 4, 128, 16, 100
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    kv, sc, bt, _ = make_cache([n], nkv, hd, page, dtype, int8, g, DEV)
+    q = torch.randn(rows, nh, hd, device=DEV, generator=g).to(dtype)
+    late = torch.arange(rows, device=DEV) >= rows // 2
+    begin, end = torch.where(late, 60, 0).int(), torch.where(late, 100, 40).int()
+
+    def run():
+        w = torch.zeros(kv.shape[0], nkv, page, device=DEV)
+        out, lse = ops.paged_attention_scored(q, kv, sc, bt, end, nkv, page, bt.shape[1] * page, begin=begin, q_len=rows, weights=w, return_lse=True)
+        return out, lse, gather_plane(w, bt, 0, n)
+
+    clean, lse0, w0 = run()
+    for t in (10, 39, 40, 50, 59):
+        blk, o = int(bt[0, t // page]), t % page
+        if int8:
+            sc[blk, :, :, o] = float("nan")
+        else:
+            kv[blk, 0, :, o], kv[blk, 1].view(nkv, hd, page)[:, :, o] = float("nan"), float("inf")
+    out, lse, w = run()
+    assert torch.equal(out[late], clean[late]) and torch.equal(lse[late], lse0[late]) and torch.equal(w[:, 40:], w0[:, 40:])
+    assert bool(torch.isnan(out[~late]).all()) and bool(torch.isnan(lse[~late]).all()) and bool(torch.isnan(w[:, :40]).all())
+
+
 @pytest.mark.parametrize("rows,track", [(1, True), (1, False), (48, True)])
 def test_graphs_and_streams(rows, track):
     """Two captured calls of different sizes, replayed in turn with eager work between, and the same calls on two streams at once: every result is the eager one, bit for bit."""
