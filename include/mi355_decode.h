@@ -390,10 +390,12 @@ int mi355_paged_attn_rows_ragged(const void* q, const mi355_kv_layer_t* kv, cons
  * A paged cache whose slots are not positions, attention with score forms over it, and eviction by attention weight.
  *
  * Two planes beside the cache, indexed as its scale plane is, [num_blocks][nkv][page]: key_pos (int32, the position of the token in a slot, per kv head,
- * as heads may keep different tokens) and weights (fp32, the attention weight that the token has drawn).  Pages of a sequence that is tracked or evicted are its own.
+ * as heads may keep different tokens) and weights (fp32, the attention weight that the token has drawn).  Pages of a sequence that is tracked or evicted are its own, each
+ * once in its row of the block table.
  *
  * mi355_rope_kv_write_slots: mi355_rope_kv_write_rows for 16-bit rows (row_seq null: row t is of sequence t / q_len, T = nseq q_len; else of row_seq[t] and q_len is 1) whose
- *   rotation goes by positions[t] (cos_sin null: no rotation, any position >= 0) and whose K / V are stored at slot slots[t] of the sequence; slots[t] < 0: a padding row.  The
+ *   rotation goes by positions[t] (cos_sin null: no rotation, any position >= 0) and whose K / V are stored at slot slots[t] of the sequence; slots[t] < 0: a padding row.  The slots
+ *   of a call differ (of rows that go to one slot any may stay, or parts of each).  The
  *   position goes to key_pos and 0 to weights there (either may be null).  A row whose position, slot, sequence or block id is out of range is not stored and counted once in oob_count.
  */
 int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias, const float* cos_sin, int32_t max_pos, const int32_t* positions,

@@ -1307,6 +1307,9 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     if (pl.few) {
+        const long np = (long)B * kv->nkv;
+        MI355_CHECK_ARG(np * (pl.ncol + (long)cdiv(max_seq_len, 256)) < (1l << 31) && (!pl.runs || np * cdiv(max_seq_len, 32) < (1l << 30)),
+                        "paged_attn_scored: %d sequences of %d slots and %d heads exceed the grid", B, max_seq_len, nh);
         p.nblocks = pl.nblocks; p.ncol = pl.ncol; p.ctx_pad = pl.ctx_pad; p.runs = pl.runs;
         p.meta = (int4*)(ws + pl.meta);
         p.tmp_out = pl.runs ? (float*)(ws + pl.tmp_out) : nullptr; p.tmp_ml = pl.runs ? (float*)(ws + pl.tmp_ml) : nullptr;

@@ -265,12 +265,13 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const EvictParams p) {
 }
 
 inline int evict_cap(int keep, int max_seq) { return std::max(0, std::min(keep, max_seq - keep)); }
+inline int evict_units(int keep, int max_seq) { return cdiv(std::min(keep, max_seq), EV_UNIT); }
 
 } // namespace
 
 extern "C" size_t mi355_kv_evict_workspace_bytes(int32_t B, int32_t nkv, int32_t keep, int32_t max_seq_len) {
     if (B <= 0 || nkv <= 0 || keep <= 0 || max_seq_len <= 0) return 0;
-    return (size_t)B * nkv * (2 + 2 * (size_t)evict_cap(keep, max_seq_len) + cdiv(keep, EV_UNIT)) * sizeof(int32_t);
+    return (size_t)B * nkv * (2 + 2 * (size_t)evict_cap(keep, max_seq_len) + evict_units(keep, max_seq_len)) * sizeof(int32_t);
 }
 
 extern "C" int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_t* key_pos, const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* seq_lens,
@@ -281,7 +282,7 @@ extern "C" int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_
     MI355_CHECK_ARG(kv->page >= 16 && kv->page % 8 == 0, "kv_evict: page=%d (>= 16, multiple of 8)", kv->page);
     MI355_CHECK_ARG(B > 0 && B <= 65535 && kv->nkv > 0 && kv->nkv <= 65535 && kv->num_blocks > 0, "kv_evict: B=%d nkv=%d num_blocks=%d", B, kv->nkv, kv->num_blocks);
     MI355_CHECK_ARG(max_seq_len > 0 && max_seq_len < (1 << 30) && max_blocks_per_seq > 0 && (long)max_blocks_per_seq * kv->page >= max_seq_len, "kv_evict: max_seq_len=%d exceeds the block table", max_seq_len);
-    MI355_CHECK_ARG((long)max_seq_len * kv->page < (1l << 32), "kv_evict: max_seq_len=%d * page=%d >= 2^32", max_seq_len, kv->page);
+    MI355_CHECK_ARG(((long)max_seq_len + EV_UNIT) * kv->page < (1l << 32), "kv_evict: (max_seq_len=%d + 64) * page=%d >= 2^32", max_seq_len, kv->page);
     MI355_CHECK_ARG(keep > 0 && sinks >= 0 && recent >= 0 && (long)sinks + recent <= keep, "kv_evict: keep=%d of which %d + %d always (keep > 0, sinks + recent <= keep)", keep, sinks, recent);
     const bool int8 = kv->kv_dtype == MI355_KV_INT8;
     MI355_CHECK_ARG(int8 || kv->kv_dtype == MI355_KV_FP16 || kv->kv_dtype == MI355_KV_BF16, "kv_evict: kv_dtype=%d", kv->kv_dtype);
@@ -297,7 +298,7 @@ extern "C" int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_
     p.new_lens = new_lens; p.max_blocks = max_blocks_per_seq; p.num_blocks = kv->num_blocks; p.nkv = kv->nkv; p.hd = kv->hd; p.page = kv->page; p.max_seq = max_seq_len;
     p.keep = keep; p.sinks = sinks; p.recent = recent; p.cap = evict_cap(keep, max_seq_len);
     p.page_magic = (uint32_t)((1ull << 32) / (unsigned)kv->page + 1);
-    p.units = cdiv(keep, EV_UNIT);
+    p.units = evict_units(keep, max_seq_len);
     p.count = (int32_t*)workspace; p.first = p.count + (size_t)B * kv->nkv; p.lists = p.first + (size_t)B * kv->nkv * (p.units + 1);
     hipStream_t st = (hipStream_t)stream;
     if (max_seq_len <= EV_KEYS) {

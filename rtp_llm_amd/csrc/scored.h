@@ -118,7 +118,8 @@ inline int scored_params(ScoredParams& p, const void* q, int ldq, const mi355_kv
     MI355_CHECK_ARG(bf || kv->act_dtype == MI355_ACT_F16, "paged_attn_scored: act_dtype=%d", kv->act_dtype);
     MI355_CHECK_ARG(int8 ? kv->scale_base != nullptr : kv->kv_dtype == (bf ? MI355_KV_BF16 : MI355_KV_FP16), "paged_attn_scored: kv_dtype=%d with act_dtype=%d (8 bits need scales, 16 bits the activations' type)",
                     kv->kv_dtype, kv->act_dtype);
-    MI355_CHECK_ARG((((uintptr_t)q | (uintptr_t)kv->kv_base | (uintptr_t)out) & 15) == 0 && (((uintptr_t)kv->scale_base) & 15) == 0, "paged_attn_scored: q, cache, scales and out lie on 16 bytes");
+    MI355_CHECK_ARG((((uintptr_t)q | (uintptr_t)kv->kv_base | (uintptr_t)out) & 15) == 0 && (((uintptr_t)kv->scale_base | (uintptr_t)sc->key_pos) & 15) == 0,
+                    "paged_attn_scored: q, cache, scales, key_pos and out lie on 16 bytes");
     MI355_CHECK_ARG(sc->softcap == 0.f || (sc->softcap >= 1e-6f && sc->softcap <= 1e6f), "paged_attn_scored: softcap=%g (0: none, or 1e-6 to 1e6)", (double)sc->softcap);
     MI355_CHECK_ARG(sc->scale > 0.f && sc->scale < 1e6f, "paged_attn_scored: scale=%g (> 0)", (double)sc->scale);
     MI355_CHECK_ARG(!sc->slopes || sc->positions, "paged_attn_scored: slopes need the rows' positions");

@@ -788,7 +788,7 @@ def rope_kv_write_slots(qkv: torch.Tensor, qkv_bias: Optional[torch.Tensor], cos
     """RoPE + bias + Q-extract + paged KV write of rows whose slot in the cache is not their position (a cache that evicts): row t is rotated at positions[t] (cos_sin None: not
     rotated, for models with distance biases) and stored at slot slots[t] of sequence t // q_len, or row_seq[t] (q_len 1); slots[t] < 0 is a padding row.  The planes key_pos (int32)
     and weights (fp32, [num_blocks, nkv, page]; see kvcache.alloc_planes) receive the position and 0.  -> q [T, nh, hd].  Rows with a position, slot, sequence or block id out of range
-    are not stored; oob_count (int32 [1]) counts them."""
+    are not stored; oob_count (int32 [1]) counts them.  No two rows of a call go to the same slot."""
     w = "rope_kv_write_slots"
     if qkv.dtype not in ACT_DTYPES or qkv.dim() != 2 or qkv.shape[1] != (nh + 2 * nkv) * hd or not qkv.is_contiguous():
         raise _C.Mi355Error(f"{w}: qkv {qkv.dtype} {tuple(qkv.shape)} for contiguous rows of ({nh} + 2 x {nkv}) heads of {hd} in float16 or bfloat16")
@@ -818,7 +818,8 @@ def paged_attention_scored(q: torch.Tensor, kv_base: torch.Tensor, scale_base: O
     Scores: softcap * tanh(scale q.k / softcap) for softcap > 0, plus slopes[h] * (key position - positions[row]) with slopes (fp32 [nh]), key positions from the plane key_pos
     (int32 [num_blocks, nkv, page]) or the slots themselves.
     weights (fp32 plane) <- decay * weights + the probabilities of the call's rows and of the heads of each kv head, for the slots below the largest end
-    of each sequence's rows that see something; kv_evict ranks by it.
+    of each sequence's rows that see something; kv_evict ranks by it.  The pages of a sequence are its own then: of one that two share, additions may be lost.
+    scale > 0, softcap 0 or 1e-6 to 1e6.  What a slot holds, infinities and NaN included, reaches the rows that see it and no others.
     The rows of q may have any stride of whole 16-byte pieces.  -> out [rows, nh * hd], with return_lse (out, log-sum-exp fp32 [rows, nh], -inf for a row that sees nothing)."""
     w = "paged_attention_scored"
     if q.dtype not in ACT_DTYPES or q.dim() != 3:

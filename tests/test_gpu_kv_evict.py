@@ -86,6 +86,44 @@ def test_blocks_out_of_the_pool_go_first_and_are_not_moved():
     run_evict([200, 120], 100, 2, 64, 16, torch.float16, False, 0, 0, spoil=spoil)
 
 
+def test_a_budget_beyond_the_cache_changes_nothing():
+    g = torch.Generator(device=DEV).manual_seed(5)
+    kv, _, bt, _ = make_cache([70, 0, 33], 2, 64, 16, torch.float16, False, g, DEV, fill=0.0)
+    w, pos = torch.rand(kv.shape[0], 2, 16, device=DEV, generator=g), torch.zeros(kv.shape[0], 2, 16, dtype=torch.int32, device=DEV)
+    lens = torch.tensor([70, 0, 33], dtype=torch.int32, device=DEV)
+    before = [x.clone() for x in (kv, w, pos)]
+    for keep in (70, 96, 1 << 30):
+        assert ops.kv_evict(w, pos, bt, lens, lens, kv, None, keep, sinks=4, recent=16).tolist() == [70, 0, 33]
+        assert all(torch.equal(a, b) for a, b in zip((kv, w, pos), before))
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_pool_of_more_than_32_bits_of_bytes(int8):
+    """Write, attend (a row and many) and evict in blocks at the far end of a large pool: as in a small one."""
+    nh, nkv, hd, page, n, far = 16, 8, 128, 16, 200, 270000 if int8 else 135000          # 8.8 GB
+    g = torch.Generator(device=DEV).manual_seed(17)
+    kv, sc, bt, _ = make_cache([n], nkv, hd, page, torch.float16, int8, g, DEV, fill=0.0)
+    nblk, used = kv.shape[0], bt[0].long()
+    w, pos = torch.rand(nblk, nkv, page, device=DEV, generator=g), torch.zeros(nblk, nkv, page, dtype=torch.int32, device=DEV)
+    qkv = torch.randn(40, (nh + 2 * nkv) * hd, device=DEV, generator=g).half()
+    big = torch.empty(far, *kv.shape[1:], dtype=kv.dtype, device=DEV)
+    big_sc = torch.zeros(far, *sc.shape[1:], device=DEV) if int8 else None
+    big_w, big_pos = torch.zeros(far, nkv, page, device=DEV), torch.zeros(far, nkv, page, dtype=torch.int32, device=DEV)
+    for a, b in ((big, kv), (big_w, w), (big_pos, pos)) + (((big_sc, sc),) if int8 else ()):
+        a[far - nblk:] = b
+    assert big.numel() * big.element_size() > 1 << 33
+    got = []
+    for c, s, wt, ps, table in ((kv, sc, w, pos, bt), (big, big_sc, big_w, big_pos, bt + (far - nblk))):
+        slots = torch.arange(n - 40, n, dtype=torch.int32, device=DEV)
+        q = ops.rope_kv_write_slots(qkv, None, None, slots, slots, table, c, s, nh, nkv, hd, page, q_len=40, key_pos=ps, weights=wt)
+        outs = [ops.paged_attention_scored(q, c, s, table, slots + 1, nkv, page, n, q_len=40, weights=wt), ops.paged_attention_scored(q[-1:], c, s, table, slots[-1:] + 1, nkv, page, n, weights=wt)]
+        lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+        new = ops.kv_evict(wt, ps, table, lens, lens, c, s, 64, sinks=4, recent=16)
+        at = table[0].long()
+        got.append(outs + [new, c[at[:4]], wt[at[:4]], ps[at[:4]]] + ([s[at[:4]]] if int8 else []))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 def test_graph_and_stream():
     """A captured eviction replayed over restored planes, with eager work between: the moves of the eager call."""
     g = torch.Generator(device=DEV).manual_seed(3)

@@ -101,6 +101,14 @@ def test_long(nh, nkv, hd, ctx, B, rows, int8):
     run_case(nh, nkv, hd, 16, torch.float16, int8, [max(0, ctx - 97 * b) for b in range(B)], [rows] * B, "causal", 30.0, None, True)
 
 
+@pytest.mark.parametrize("nh,nkv,int8", [(4, 1, False), (8, 4, False), (8, 4, True)])
+@pytest.mark.parametrize("rows", [1, 2])
+def test_many_short_sequences(nh, nkv, int8, rows):
+    """300 sequences, some without tokens or rows: in runs that cross sequences (one kv head), and a block for each pair (four)."""
+    ctx = [(37 * b) % 211 if b % 5 else 0 for b in range(300)]
+    run_case(nh, nkv, 64, 16, torch.float16, int8, ctx, [0 if b % 7 == 3 else 1 + b % rows for b in range(300)], "window", 0.0, None, True)
+
+
 def test_large_scores_and_late_maxima():
     """Scores that grow along the keys (the running maximum moves all the time) and reach hundreds, capped and not."""
     for cap in (0.0, 50.0):

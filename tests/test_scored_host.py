@@ -33,6 +33,21 @@ def test_attention_refuses(kw, said):
     assert said.encode() in _C.lib().mi355_last_error(), _C.lib().mi355_last_error()
 
 
+@pytest.mark.parametrize("kw,said", [
+    (dict(score=_C.AttnScore(0.0, 0.0, None, None, None, None, 16)), "scale=0"), (dict(score=_C.AttnScore(-0.1, 0.0, None, None, None, None, 16)), "scale=-0.1"),
+    (dict(score=_C.AttnScore(float("nan"), 0.0, None, None, None, None, 16)), "scale"), (dict(score=_C.AttnScore(0.1, 1e-7, None, None, None, None, 16)), "softcap"),
+    (dict(score=_C.AttnScore(0.1, 0.0, 16, 16, 24, None, 16)), "16 bytes"), (dict(ws=24), "16 bytes"), (dict(B=2048, rows=2048, nh=1 << 10, ldq=1 << 17, kv=_kv(nkv=1 << 10), M=1 << 20, most=1 << 24), "grid")])
+def test_attention_refuses_scales_addresses_and_grids(kw, said):
+    assert _attend(**dict(dict(nbytes=1 << 62), **kw)) == _C.ERR_ARG
+    assert said.encode() in _C.lib().mi355_last_error(), _C.lib().mi355_last_error()
+
+
+def test_eviction_needs_nothing_for_a_budget_that_no_sequence_reaches():
+    need = _C.lib().mi355_kv_evict_workspace_bytes
+    assert need(4, 8, 1 << 30, 4096) == need(4, 8, 4096, 4096) < 1 << 16
+    assert _evict(M=1 << 26, most=(1 << 28) - 16) == _C.ERR_ARG and b"2^32" in _C.lib().mi355_last_error()
+
+
 def test_attention_refuses_a_short_workspace():
     assert _C.lib().mi355_paged_attn_scored_workspace_bytes(1, 1, 1, 28, 4, 128, 64, 1) > 0
     assert _attend(weights=16, nbytes=0) == _C.ERR_WORKSPACE and _attend(weights=16, ws=None) == _C.ERR_WORKSPACE
