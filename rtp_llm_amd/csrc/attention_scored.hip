@@ -979,50 +979,53 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
     }
 }
 
-// Parts of the keys into results: a wave per column.
+// Parts of the keys into results: 16 bytes a thread, HD / 4 threads a column, eight parts in flight.
 template <int HD, bool BF>
 __global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) {
-    const int lane = threadIdx.x & 63;
-    const size_t cols = (size_t)p.rows * p.G, at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= cols * p.nkv) return;
-    const int kh = (int)(at / cols), c = (int)(at - kh * cols), row = c / p.G, h = kh * p.G + c - row * p.G;
-    constexpr int CPL = HD / 64;
-    float m = NEG_BIG, l = 0.f, acc[CPL];
+    constexpr int TP = HD / 4;
+    const int d0 = threadIdx.x % TP * 4;
+    const size_t cols = (size_t)p.rows * p.G, all = cols * p.nkv, at = (size_t)blockIdx.x * (256 / TP) + threadIdx.x / TP;
+    if (at >= all) return;
+    float m = NEG_BIG, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     int ref = 0;
+    for (int i0 = 0; i0 < p.parts; i0 += 8) {
+        float4 ml[8];
+        f32x4 v[8];
 #pragma unroll
-    for (int k = 0; k < CPL; ++k) acc[k] = 0.f;
-    int b = row / p.q_len;
+        for (int i = 0; i < 8; ++i) {
+            const size_t slot = min(i0 + i, p.parts - 1) * all + at;
+            ml[i] = p.tmp_ml[slot];
+            v[i] = *reinterpret_cast<const f32x4*>(p.tmp_out + slot * HD + d0);
+        }
+        ref = __builtin_bit_cast(int, ml[0].z);
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn);
+        l *= f0; acc *= f0; m = mn;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= p.parts) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - m);
+            l += ml[i].y * f;
+            acc += v[i] * f;
+        }
+    }
+    const int kh = (int)(at / cols), c = (int)(at - kh * cols), row = c / p.G, h = kh * p.G + c - row * p.G;
     if (p.row_start) {                              // the row's sequence; a row behind the last has no parts
         int lo = 0, hi = p.B;
         while (lo < hi) { const int mid = (lo + hi) >> 1; if (p.row_start[mid + 1] > row) hi = mid; else lo = mid + 1; }
-        b = lo;
-        if (b >= p.B) return;
+        if (lo >= p.B) return;
         int base, len;
-        scored_rows_of(p, b, base, len);
+        scored_rows_of(p, lo, base, len);
         if (row < base || row >= base + len) return;
-    }
-    const int np = p.parts;
-    for (int i = 0; i < np; ++i) m = fmaxf(m, p.tmp_ml[i * cols * p.nkv + at].x);
-    for (int i = 0; i < np; ++i) {
-        const size_t slot = i * cols * p.nkv + at;
-        const float4 ml = p.tmp_ml[slot];
-        ref = __builtin_bit_cast(int, ml.z);
-        const float f = __builtin_amdgcn_exp2f(ml.x - m);
-        l += ml.y * f;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) acc[k] += p.tmp_out[slot * HD + lane * CPL + k] * f;
     }
     int a, e;
     scored_interval(p, row, a, e);
     const bool seen = e > a;
-    const float inv = scored_inv(l, seen);
-    uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + ((size_t)row * p.nh + h) * HD + lane * CPL;
-#pragma unroll
-    for (int k = 0; k < CPL; ++k) dst[k] = act_to_bits<BF>(seen ? acc[k] * inv : 0.f);
-    if (lane == 0) {
-        if (p.lse) p.lse[(size_t)row * p.nh + h] = scored_lse(m, l, seen, seen ? scored_shift(p, row, h, ref) : 0.f);
-        if (p.cols) p.cols[at] = Col{m, inv, p.slopes ? p.slopes[h] * kLog2e : 0.f, ref, a, e, 0, 0};
-    }
+    scored_store<BF>(p, row, h, HD, d0, acc, m, l, seen, ref);
+    if (p.cols && d0 == 0) p.cols[at] = Col{m, scored_inv(l, seen), p.slopes ? p.slopes[h] * kLog2e : 0.f, ref, a, e, 0, 0};
 }
 
 // The weights of many rows: S^T once more, a wave's 64 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 256 keys, its 8 waves the two halves of
@@ -1270,7 +1273,7 @@ int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
            : pl.waves == 4 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 4>, Stage<HD, INT8, 4>::LDS, 256, blocks)
                            : run(scored_chunk_kernel<HD, INT8, BF, FORM, 8>, Stage<HD, INT8, 8>::LDS, 512, blocks);
     if (rc != MI355_OK) return rc;
-    if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 3) / 4)), dim3(256), 0, st, c);
+    if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 1024 / HD - 1) / (1024 / HD))), dim3(256), 0, st, c);
     if (c.weights) {
         const int key_tiles = cdiv(c.max_seq, 256);
         rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 3 * (128 * HD * 2 + 4096) + 16, 512, (long)key_tiles * c.nkv * c.B * pl.splits, key_tiles, pl.splits);
