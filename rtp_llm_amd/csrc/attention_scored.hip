@@ -56,6 +56,7 @@ __device__ __forceinline__ u32x4 seen_big(int t, int lo, int hi) {
 // Work: the tokens that any row of a sequence sees, in units of a group of 32 for each of a block's waves, times key/value heads, laid end to end over all sequences and dealt to the
 // blocks in equal runs.  A pair of a sequence and a head that lies inside one run is finished there, others leave a part in each run and scored_join_kernel merges them.  Sequences
 // of unequal length so take the time of their mean: a run may end one pair and begin the next.
+// Bound by memory: 64 sequences of up to 1024 tokens (28 over 4 heads of 128, 80 MB) 21 us, 3.7 TB/s, where a sum over a large array reads 4.0; one row over one short sequence is latency, 7 us.
 struct DecodeParams : ScoredParams {
     float*   tmp_out;    // [2 nblocks][ncol][hd]: parts; a run's first segment in slot 2 run, a later one that goes on in the next run in 2 run + 1
     float*   tmp_ml;     // [2 nblocks][ncol][2]
@@ -601,6 +602,8 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
 // 16 (i / 2) + 8 half + 4 (i & 1) + r for row 8 i + 4 half + r: what a lane then holds of its column are two runs of eight keys, the second product's operand as it stands.
 // Keys and values come 64 at a time through LDS for all waves: by DMA, two steps ahead of the products with one barrier a step (three stages), or, 8 bits, through registers, which widen them
 // once for all waves.  A key's 16-byte pieces are swizzled by its low bits, a channel's 16 tokens lie side by side: no bank conflicts in either product's reads.
+// 28 heads of 128: 2 x 2048 rows behind 2048 slots 227 us (0.79 PFLOP/s), 4096 behind 12288 916 us (0.92), 8 x 512 capped 47 us.  Products take 43% of the busy time of a compute unit in the
+// first of these, vector instructions 44%: what is left is waiting, of the two kinds for each other in a wave and at a step's barrier.
 // What the weights' pass needs of a column.
 struct Col { float m, inv, slope2; int ref, lo, hi, pad0, pad1; };
 static_assert(sizeof(Col) == 32, "two 16-byte loads");
@@ -1029,8 +1032,11 @@ __global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) 
 }
 
 // The weights of many rows: S^T once more, a wave's 64 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 256 keys, its 8 waves the two halves of
-// 128 columns at a time (three stages of DMA); a probability is added in the lane of its column, lanes and halves meet once at the end: no atomics, the same sums every time.  Keys that
-// all rows see take longer than late ones: where blocks are few the columns are dealt to `splits` blocks and scored_decay_kernel adds their shares.
+// 128 columns at a time (three stages of DMA); a probability is added in the lane of its column, lanes and halves meet once at the end: no atomics, the same sums every time.  A block's
+// columns are those of the rows between the first and the last that see some of its keys; tiles that most rows see come first; where blocks are few the columns are dealt to `splits` blocks
+// and scored_decay_kernel adds their shares.  2 x 2048 rows of 28 heads behind 2048 slots: 169 us, 0.53 PFLOP/s of products; compute units are busy for 85% of it, vector
+// instructions, the exponentials first, take 53% of that time and products 30%.  (Products of the next 32 columns laid among the exponentials of the last ones: 181 us against 170 then, the
+// registers' copies took more.)
 template <int HD, bool INT8, bool BF, int FORM>
 __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p, int key_tiles, int splits) {
     constexpr int KS = HD / 16, ROW = HD * 2, CK = ROW / 16, QB = 128 * ROW, SB = QB + 4096, LOADS = QB / 1024, JL = LOADS / 8, NS = 3;
@@ -1039,13 +1045,12 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
     int* s_reach = reinterpret_cast<int*>(su_sm + NS * SB);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5, cg = wave >> 2;
     int id = blockIdx.x;
-    const int tile = id % key_tiles; id /= key_tiles;                // early keys, which most rows see, first
     const int kh = id % p.nkv; id /= p.nkv;
-    const int b = id % p.B, split = id / p.B;
+    const int b = id % p.B; id /= p.B;
+    const int split = id % splits, tile = id / splits;               // early keys, which most rows see, first
     int base, len;
     scored_rows_of(p, b, base, len);
     const int ncol = len * p.G, tw = tile * 256 + (wave & 3) * 64;    // the wave's first slot
-    const int all = (ncol + 127) / 128, st0 = (int)((long)all * split / splits), st1 = (int)((long)all * (split + 1) / splits);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)su_sm;
     const char* cols = reinterpret_cast<const char*>(p.cols + (size_t)kh * p.rows * p.G + (size_t)base * p.G);
     auto issue = [&](int st, int buf) {
@@ -1058,25 +1063,28 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
         if (wave < 4)                                                // 32 columns' facts a load (the last, past the sequence's, are its last one's: not looked at)
             dma16(__builtin_amdgcn_readfirstlane(lds0 + buf * SB + QB + wave * 1024), cols + (size_t)min(st * 128 + wave * 32 + (lane >> 1), ncol - 1) * 32 + (lane & 1) * 16);
     };
-    if (st0 < st1) issue(st0, 0);
-    if (st0 + 1 < st1) issue(st0 + 1, 1);
-    if (tid == 0) *s_reach = 0;
-    lds_barrier();
-    int reach = 0;
-    for (int i = tid; i < len; i += 512) { int a, e; scored_interval(p, base + i, a, e); reach = max(reach, e); }
-    reach = row32(reach, [](int a, int c) { return max(a, c); });
-    if ((lane & 31) == 0) atomicMax(s_reach, reach);
-    lds_barrier();
-    reach = __builtin_amdgcn_readfirstlane(*s_reach);
-    if (splits > 1 && tile == 0 && kh == 0 && split == 0 && tid == 0) p.reach[b] = reach;
-    if (tile * 256 >= reach) { wait_vm<0>(); return; }               // the loads above must not land in another block's LDS
+    // the last slot that any row sees, and the rows [r0, r1) between which all lie that see some of the tile: their columns are the block's
+    if (tid == 0) { s_reach[0] = 0; s_reach[1] = 0x7fffffff; s_reach[2] = 0; }
+    int reach = 0, r0 = 0x7fffffff, r1 = 0;
+    for (int i0 = tid; i0 < len; i0 += 4 * 512) {
+        int a[4], e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) scored_interval(p, base + min(i0 + j * 512, len - 1), a[j], e[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = min(i0 + j * 512, len - 1);
+            reach = max(reach, e[j]);
+            if (e[j] > tile * 256 && a[j] < tile * 256 + 256) { r0 = min(r0, i); r1 = max(r1, i + 1); }
+        }
+    }
+    // the wave's keys, on their way during the reductions
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
     u32x4 kfr[2][KS];
     float ksc[INT8 ? 2 : 1][INT8 ? 16 : 1];
     i32x4 kp[FORM == FORM_BIAS ? 2 : 1][FORM == FORM_BIAS ? 4 : 1];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        const int t = min(tw + g * 32 + col, reach - 1), blk = scored_block(p, bt, t);
+        const int t = min(tw + g * 32 + col, p.max_seq - 1), blk = scored_block(p, bt, t);
         const size_t at = (((size_t)blk * 2) * p.nkv + kh) * p.page + t % p.page;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -1087,7 +1095,7 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {                                // the lane's results are keys 8 i + 4 half + r
-            const int tt = tw + g * 32 + i * 8 + half * 4, tc = min(tt, (reach - 1) & ~3), bl = scored_block(p, bt, tc);
+            const int tt = tw + g * 32 + i * 8 + half * 4, tc = min(tt, (p.max_seq - 1) & ~3), bl = scored_block(p, bt, tc);
             if constexpr (INT8) {
                 const f32x4 v = *reinterpret_cast<const f32x4*>(p.scale_base + (((size_t)bl * 2) * p.nkv + kh) * p.page + tc % p.page);
 #pragma unroll
@@ -1099,6 +1107,18 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
             }
         }
     }
+    const auto larger = [](int a, int c) { return max(a, c); };
+    reach = row32(reach, larger); r1 = row32(r1, larger); r0 = row32(r0, [](int a, int c) { return min(a, c); });
+    lds_barrier();
+    if ((lane & 31) == 0) { atomicMax(&s_reach[0], reach); atomicMin(&s_reach[1], r0); atomicMax(&s_reach[2], r1); }
+    lds_barrier();
+    reach = __builtin_amdgcn_readfirstlane(s_reach[0]); r0 = __builtin_amdgcn_readfirstlane(s_reach[1]); r1 = __builtin_amdgcn_readfirstlane(s_reach[2]);
+    if (splits > 1 && tile == 0 && kh == 0 && split == 0 && tid == 0) p.reach[b] = reach;
+    if (tile * 256 >= reach) return;
+    const int first = r1 > 0 ? r0 * p.G / 128 : 0, all = r1 > 0 ? (r1 * p.G + 127) / 128 - first : 0;
+    const int st0 = first + (int)((long)all * split / splits), st1 = first + (int)((long)all * (split + 1) / splits);
+    if (st0 < st1) issue(st0, 0);
+    if (st0 + 1 < st1) issue(st0 + 1, 1);
     float acc[2][16];
 #pragma unroll
     for (int g = 0; g < 2; ++g)
@@ -1170,14 +1190,19 @@ __global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p
             }
         }
     }
-    float sum = 0.f;                                                 // lane `col` ends up with result `col`: 16 of each group
+    float sums[32];                                                  // over the 32 lanes: lane `col` ends up with result `col`, 16 of each group; at every step half the results go over
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        float v = acc[i >> 4][i & 15];
+    for (int i = 0; i < 32; ++i) sums[i] = acc[i >> 4][i & 15];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) v += __shfl_xor(v, o);
-        if (col == i) sum = v;
-    }
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            float a = sums[i], e = sums[i + o];
+            asm("" : "+v"(a), "+v"(e));                              // two registers, not an index that a lane looks up
+            const float keep = col & o ? e : a, give = col & o ? a : e;
+            sums[i] = keep + __shfl_xor(give, o);
+        }
+    float sum = sums[0];
     __syncthreads();
     const int key = (wave & 3) * 64 + (col >> 4) * 32 + (col >> 2 & 3) * 8 + half * 4 + (col & 3);
     if (cg > 0) meet[key] = sum;
@@ -1232,9 +1257,9 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         if (track) { pl.ml_all = region(pairs * pl.ncol * 8); pl.spill = region(pairs * pl.ncol * pl.ctx_pad * 4); }
     } else {
         const long cols = (long)q_len * G;
-        // Four waves a block, two blocks a compute unit: one fills in while the other one starts, ends or waits.  us by eight / by four: 16 x 64 rows 12.8 / 10.4, 4 x 512 34 / 30, 32 x 512
-        // 154 / 139, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 895 / 952) and
-        // where keys and values are widened on the way (333 rows behind 3001 46 / 53).
+        // Four waves a block, two blocks a compute unit: one fills in while the other one starts, ends or waits.  us by eight / by four: 16 x 64 rows 13.0 / 10.5, 4 x 512 29 / 25, 32 x 512
+        // 157 / 144, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 916 / 946) and
+        // where keys and values are widened on the way (333 rows behind 3001 47 / 60).
         pl.waves = cols <= 64 ? 2 : cols <= 128 || (!int8 && max_seq < 8192) ? 4 : 8;
         pl.tiles = (int)((cols + 32 * pl.waves - 1) / (32 * pl.waves));
         const long blocks = (long)pl.tiles * B * nkv, room = 256 * 8 / pl.waves;
@@ -1243,7 +1268,7 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         if (track) {
             pl.ml_all = region((size_t)rows * nh * sizeof(Col));
             const long kb = (long)cdiv(max_seq, 256) * nkv * B;
-            pl.splits = (int)std::max(1l, std::min({512 / kb, (cols + 1023) / 1024, 4l}));
+            pl.splits = (int)std::max(1l, std::min({1024 / kb, (cols + 1023) / 1024, 8l}));     // at least 8 steps each; us for 2 x 2048 rows behind 2048 by 2 / 4 / 8: 175 / 179 / 169, at best 159 / 165 / 155
             if (pl.splits > 1) pl.spill = region(((size_t)pl.splits * nkv * max_seq + 1) * B * 4);
         }
     }
