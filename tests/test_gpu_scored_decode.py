@@ -80,6 +80,43 @@ def test_steps_of_a_cache_with_a_budget(dtype, nh, nkv, hd, page, form):
     assert moved > 100
 
 
+@pytest.mark.parametrize("int8", [False, True])
+def test_captured_steps(int8):
+    """A step's write, attention and eviction in one graph, replayed step after step with eager work between: bit for bit the eager chain on a cache of its own."""
+    dtype, nh, nkv, hd, page, B, budget = torch.float16, 16, 4, 128, 16, 3, 24
+    c = AttentionConfigs(nh, nkv, hd, rope_dim=hd, max_seq_len=64, kv_budget=budget, kv_sinks=2, kv_recent=6, softcap=20.0)
+    ang = torch.arange(128, device=DEV, dtype=torch.float64)[:, None] * 0.7 ** torch.arange(hd // 2, device=DEV, dtype=torch.float64)
+    cs = torch.stack([ang.cos(), ang.sin()], -1).float()
+    bt = torch.randperm(B * 4 + 1, generator=torch.Generator().manual_seed(2))[: B * 4].reshape(B, 4).int().to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    caches = []
+    for _ in range(2):
+        kv, sc = kvcache.alloc_layer_cache(B * 4 + 1, nkv, page, hd, int8, DEV, dtype)
+        kv.zero_()
+        if sc is not None:
+            sc.zero_()
+        caches.append(LayerKVCache(kv, sc, page, 0, *kvcache.alloc_planes(B * 4 + 1, nkv, page, DEV)))
+    lens, positions = torch.tensor([0, 0, 0], dtype=torch.int32), torch.tensor([0, 3, 1], dtype=torch.int32)
+    qkv = torch.zeros(B, (nh + 2 * nkv) * hd, device=DEV, dtype=dtype)
+    inputs = lambda: PyAttentionInputs(sequence_lengths=lens, kv_cache_kernel_block_id_device=bt, token_positions=positions, is_cuda_graph=True)
+    impl, gr = AttnImplFactory.get_fmha_impl(c, inputs(), cos_sin=cs), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):                                               # nothing runs here
+        out = impl.forward(qkv, caches[0])
+        new = impl.evict(caches[0])
+    for step in range(60):
+        qkv.copy_(torch.randn(qkv.shape, device=DEV, generator=g))
+        impl.prepare_cuda_graph(inputs())
+        gr.replay()
+        eager = AttnImplFactory.get_fmha_impl(c, inputs(), cos_sin=cs)
+        want = eager.forward(qkv, caches[1])
+        want_new = eager.evict(caches[1])
+        assert torch.equal(out, want) and torch.equal(new, want_new) and new.tolist() == [min(step + 1, budget)] * B, step
+        a, b = caches
+        assert torch.equal(a.kv_cache_base, b.kv_cache_base) and torch.equal(a.weights, b.weights) and torch.equal(a.key_pos, b.key_pos), step
+        assert not int8 or torch.equal(a.kv_scale_base, b.kv_scale_base)
+        lens, positions = new.cpu(), positions + 1
+
+
 def test_plain_configurations_keep_their_implementation():
     inputs = PyAttentionInputs(sequence_lengths=torch.tensor([3]), kv_cache_kernel_block_id_device=torch.zeros(1, 2, dtype=torch.int32, device=DEV))
     assert type(AttnImplFactory.get_fmha_impl(AttentionConfigs(8, 2, 64), inputs)) is Mi355PagedDecodeImpl
