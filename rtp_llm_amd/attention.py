@@ -141,7 +141,8 @@ class Mi355ScoredDecodeImpl(Mi355PagedDecodeImpl):
             raise ValueError("a cache with a budget needs its planes (kvcache.alloc_planes)")
         q = ops.rope_kv_write_slots(qkv.contiguous(), None, None if c.slopes is not None else self.cos_sin, self.positions, self.slots, self.block_table, kv_cache.kv_cache_base,
                                     kv_cache.kv_scale_base, c.head_num, c.kv_head_num, c.size_per_head, page, key_pos=kv_cache.key_pos, weights=kv_cache.weights)
-        return ops.paged_attention_scored(q, kv_cache.kv_cache_base, kv_cache.kv_scale_base, self.block_table, self.seq_lens, c.kv_head_num, page, c.max_seq_len,
+        # slots are bounded by the block table, as evict() has them, not by max_seq_len: that is of positions, and a budget's table may be shorter
+        return ops.paged_attention_scored(q, kv_cache.kv_cache_base, kv_cache.kv_scale_base, self.block_table, self.seq_lens, c.kv_head_num, page, self.block_table.shape[1] * page,
                                           scale=c.softmax_extra_scale / math.sqrt(c.size_per_head), softcap=c.softcap, slopes=c.slopes,
                                           positions=self.positions if c.slopes is not None else None, key_pos=kv_cache.key_pos if c.slopes is not None else None,
                                           weights=kv_cache.weights if c.kv_budget > 0 else None, decay=c.kv_decay)

@@ -1,0 +1,46 @@
+"""What the scored decode implementation hands to its operators, on the host: the bound on slots, the rotation, the planes."""
+import pytest
+import torch
+
+from rtp_llm_amd import kvcache
+from rtp_llm_amd import attention as A
+
+NH, NKV, HD, PAGE = 8, 2, 64, 16
+
+
+def impl_of(monkeypatch, calls, *, table_blocks, lens, positions=None, cos_sin=None, **cfg):
+    """An implementation whose operators only note their arguments."""
+    def write(qkv, bias, cos, pos, slots, *a, **kw):
+        calls.append(("write", cos, pos.clone(), slots.clone(), kw))
+        return qkv.view(qkv.shape[0], -1, HD)[:, :NH]
+
+    def attend(q, kv, sc, bt, end, nkv, page, most, **kw):
+        calls.append(("attend", most, end.clone(), kw))
+        return q.reshape(q.shape[0], -1)
+
+    def evict(w, pos, bt, lens, nxt, kv, sc, keep, **kw):
+        calls.append(("evict", bt.shape[1] * PAGE if kw.get("max_seq_len") is None else kw["max_seq_len"], lens.clone(), nxt.clone(), keep))
+        return lens.clamp(max=keep)
+
+    for name, f in (("rope_kv_write_slots", write), ("paged_attention_scored", attend), ("kv_evict", evict)):
+        monkeypatch.setattr(A.ops, name, f)
+    inputs = A.PyAttentionInputs(sequence_lengths=lens, kv_cache_kernel_block_id_device=torch.zeros(len(lens), table_blocks, dtype=torch.int32), token_positions=positions)
+    return A.AttnImplFactory.get_fmha_impl(A.AttentionConfigs(NH, NKV, HD, **cfg), inputs, cos_sin=cos_sin)
+
+
+def cache(planes=True):
+    w, pos = kvcache.alloc_planes(8, NKV, PAGE, "cpu") if planes else (None, None)
+    return A.LayerKVCache(torch.zeros(8, 2, NKV, PAGE, HD, dtype=torch.float16), None, PAGE, 0, w, pos)
+
+
+@pytest.mark.parametrize("table_blocks,max_seq_len", [(3, 4096), (300, 4096)])
+def test_slots_are_bounded_by_the_table(monkeypatch, table_blocks, max_seq_len):
+    """max_seq_len bounds positions.  A budget's table may be shorter, and a longer one's slots are all written, attended and ranked."""
+    calls = []
+    impl = impl_of(monkeypatch, calls, table_blocks=table_blocks, lens=torch.tensor([30, 47]), positions=torch.tensor([2000, 4000]), cos_sin=torch.zeros(4096, HD // 2, 2), rope_dim=HD,
+                   max_seq_len=max_seq_len, kv_budget=32, kv_sinks=2, kv_recent=8)
+    impl.forward(torch.zeros(2, (NH + 2 * NKV) * HD, dtype=torch.float16), cache())
+    impl.evict(cache())
+    (_, _, pos, slots, _), (_, most, end, _), (_, ranked, lens, nxt, keep) = calls
+    assert most == ranked == table_blocks * PAGE
+    assert slots.tolist() == [30, 47] and pos.tolist() == [2000, 4000] and end.tolist() == lens.tolist() == [31, 48] and nxt.tolist() == [2001, 4001] and keep == 32
