@@ -117,6 +117,12 @@ class Mi355ScoredDecodeImpl(Mi355PagedDecodeImpl):
     """The same pairing for capped or biased scores and for a cache with a budget: the writer puts a token at the next slot, whatever its position, the attention adds up what every cached token
     draws, and evict() brings the cache back to the budget."""
 
+    def __init__(self, attn_configs: AttentionConfigs, attn_inputs: PyAttentionInputs, parallelism_config=None, cos_sin: Optional[torch.Tensor] = None, qkv_bias: Optional[torch.Tensor] = None):
+        # no table means no rotation to the writer: that has to be the model's choice (slopes, or no rotated channels)
+        if attn_configs.slopes is None and attn_configs.rope_dim != 0 and cos_sin is None:
+            raise ValueError(f"rope_dim={attn_configs.rope_dim} needs cos_sin (models with slopes do not rotate)")
+        super().__init__(attn_configs, attn_inputs, parallelism_config, cos_sin, qkv_bias)
+
     @staticmethod
     def support(attn_configs: AttentionConfigs, attn_inputs: PyAttentionInputs) -> bool:
         return (not attn_inputs.is_prefill and attn_configs.scored and attn_configs.size_per_head in (64, 128) and attn_configs.head_num % max(1, attn_configs.kv_head_num) == 0

@@ -44,3 +44,18 @@ def test_slots_are_bounded_by_the_table(monkeypatch, table_blocks, max_seq_len):
     (_, _, pos, slots, _), (_, most, end, _), (_, ranked, lens, nxt, keep) = calls
     assert most == ranked == table_blocks * PAGE
     assert slots.tolist() == [30, 47] and pos.tolist() == [2000, 4000] and end.tolist() == lens.tolist() == [31, 48] and nxt.tolist() == [2001, 4001] and keep == 32
+
+
+def test_rotated_models_need_the_rotation(monkeypatch):
+    """No table means no rotation to the writer: a model that rotates is refused without one, one with slopes or without rotated channels runs."""
+    table, lens = torch.zeros(64, HD // 2, 2), torch.tensor([3])
+    for cfg in (dict(softcap=30.0), dict(kv_budget=40), dict(softcap=30.0, kv_budget=40)):
+        with pytest.raises(ValueError, match="cos_sin"):
+            impl_of(monkeypatch, [], table_blocks=4, lens=lens, rope_dim=HD, **cfg)
+        calls = []
+        impl_of(monkeypatch, calls, table_blocks=4, lens=lens, rope_dim=HD, cos_sin=table, **cfg).forward(torch.zeros(1, (NH + 2 * NKV) * HD, dtype=torch.float16), cache())
+        assert calls[0][1] is table
+    for cfg in (dict(slopes=torch.ones(NH), rope_dim=HD), dict(softcap=30.0, rope_dim=0), dict(slopes=torch.ones(NH), rope_dim=0)):
+        calls = []
+        impl_of(monkeypatch, calls, table_blocks=4, lens=lens, **cfg).forward(torch.zeros(1, (NH + 2 * NKV) * HD, dtype=torch.float16), cache())
+        assert calls[0][1] is None
