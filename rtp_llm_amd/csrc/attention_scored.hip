@@ -534,6 +534,7 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
     }
     // ---- weights: SL slots a thread, the first scores asked for before the columns' maxima and sums are merged
     __shared__ float s_m[32], s_i[32];
+    __shared__ int2 s_seen[32];                                      // what a column sees: by the score alone a slot of -inf were one that it does not see, and a column that is not a number passed it over
     typedef float slots __attribute__((ext_vector_type(SL)));
     const int id = blockIdx.x - join_blocks, pair = id / chunks, chunk = id - pair * chunks;
     const int4 mt = p.meta[pair];
@@ -569,7 +570,7 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
         }
         int a, e;
         scored_interval(p, base + col / p.G, a, e);
-        if (lane == 0) { s_m[col] = m; s_i[col] = scored_inv(l, e > a); }
+        if (lane == 0) { s_m[col] = m; s_i[col] = scored_inv(l, e > a); s_seen[col] = make_int2(a, e); }
     }
     __syncthreads();
     if (!in || blk < 0 || blk >= p.num_blocks) return;
@@ -583,8 +584,9 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
             for (int i = 0; i < 8; ++i) {
                 if (c0 + i >= ncol) continue;
                 const float m = s_m[c0 + i], inv = s_i[c0 + i];
+                const int2 seen = s_seen[c0 + i];
 #pragma unroll
-                for (int e = 0; e < SL; ++e) sum[e] += v[i][e] <= NEG_BIG || inv == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[i][e] - m) * inv;
+                for (int e = 0; e < SL; ++e) sum[e] += t + e >= seen.x && t + e < seen.y ? __builtin_amdgcn_exp2f(v[i][e] - m) * inv : 0.f;
             }
             if (c0 + 8 < ncol) {
 #pragma unroll

@@ -1,0 +1,47 @@
+"""Edges of scored attention, tracked writes and eviction: scores that are all -inf."""
+import pytest
+import torch
+
+from rtp_llm_amd import ops
+from tests.scored_util import attend, bounds, gather_plane, make_cache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [(torch.float16, False), (torch.bfloat16, False), (torch.float16, True), (torch.bfloat16, True)]
+
+
+def weight_bound(w, old, rel, terms, rows):
+    """As the attention's other tests: each probability is off by rel, the sum of `terms` rounds at each, decay and addition once each, and what lies below 2^-60 of one may be lost."""
+    return w * (rel + terms * 2.0 ** -24) + 2.0 ** -22 * (old + w) + rows * 2.0 ** -60
+
+
+@pytest.mark.parametrize("dtype,int8", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 128), (6, 2, 64)])
+@pytest.mark.parametrize("rows", [2, 5, 40, 700])
+def test_scores_that_are_all_minus_infinity(nh, nkv, hd, dtype, int8, rows):
+    """Row 0 sees slots 20 to 23 alone, whose scores are -inf: a softmax of these is not a number, in its output and in the weights of the slots it sees, and nowhere else.  The other rows see all
+    slots: their shares of 20 to 23 are 0."""
+    n, page = 60, 16
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    kv, sc, bt, dense = make_cache([n], nkv, hd, page, dtype, int8, g, DEV)
+    q = (torch.randn(rows, nh, hd, device=DEV, generator=g).abs() + 0.1).to(dtype)        # positive, the four keys negative: no inf - inf inside a score
+    for t in range(20, 24):
+        blk, o = int(bt[0, t // page]), t % page
+        if int8:
+            kv[blk, 0, :, o], sc[blk, 0, :, o] = 127, float("inf")                         # the stored byte of the code -1
+        else:
+            kv[blk, 0, :, o], kv[blk, 0, :, o, 3] = -1.0, float("-inf")
+    begin, end = torch.zeros(rows, dtype=torch.int32, device=DEV), torch.full((rows,), n, dtype=torch.int32, device=DEV)
+    begin[0], end[0] = 20, 24
+    w = torch.full((kv.shape[0], nkv, page), 0.5, device=DEV)
+    out, lse = ops.paged_attention_scored(q, kv, sc, bt, end, nkv, page, bt.shape[1] * page, begin=begin, q_len=rows, weights=w, return_lse=True)
+    out, got = out.view(rows, nh, hd).double(), gather_plane(w, bt, 0, n).double()
+    others = torch.tensor([t for t in range(n) if not 20 <= t < 24], device=DEV)
+    k, v = (x[:, others].contiguous() for x in dense[0])
+    ref, ref_lse, want, pv, size = attend(q[1:], k, v, torch.zeros(rows - 1, device=DEV), torch.full((rows - 1,), n, device=DEV), scale=hd ** -0.5)
+    t_out, t_lse, rel = bounds(dtype, hd, n, pv, size, ref)
+    assert bool(torch.isnan(out[0]).all()) and not bool(torch.isfinite(lse[0]).any())
+    assert bool(((out[1:] - ref).abs() <= t_out).all()) and bool(((lse[1:].double() - ref_lse).abs() <= t_lse + 2.0 ** -22 * ref_lse.abs()).all())
+    assert bool(torch.isnan(got[:, 20:24]).all())
+    t_w = weight_bound(want, 0.5, float(rel.max()), rows * nh // nkv, rows)
+    assert bool(((got[:, others] - 0.5 - want).abs() <= t_w).all())
