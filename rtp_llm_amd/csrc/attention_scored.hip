@@ -78,6 +78,9 @@ __device__ __forceinline__ void scored_span(const ScoredParams& p, int base, int
     lo = hi == 0 ? 0 : seen & ~31;
 }
 
+// a row's reference of biases where the thread writes its log-sum-exp
+__device__ __forceinline__ int lse_ref(const ScoredParams& p, int b, int kh, int d0, int hi) { return p.slopes && p.lse && d0 == 0 && hi > 0 ? scored_ref(p, b, kh, hi) : 0; }
+
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // 8 cache bytes (code + 128) -> the codes, exact in both types.  With the offset left inside (1152 under fp16's exponent of 1024, 128 in bf16) and taken out of the sums behind the products,
@@ -204,7 +207,6 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
         const int pstart = lo + u * UNIT, pend = min(hi, lo + stop_u * UNIT);
         const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
         const size_t pair = (size_t)b * p.nkv + kh;
-        const int ref = p.slopes ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, hi)) : 0;
 
         // the first groups' block ids are asked for together with the queries
         const int last16 = (hi - 1) & ~15;
@@ -215,7 +217,7 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
         };
         ids_of(0);
         u32x4 qf[NT][NSTEP];
-        int c_lo[NT], c_hi[NT];
+        int c_lo[NT], c_hi[NT], ref[NT];
         float slope2[NT];
         int in_lo = 0, in_hi = 0x7fffffff;          // every column of this lane sees [in_lo, in_hi)
 #pragma unroll
@@ -227,6 +229,7 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
             if (!ok) c_lo[c] = c_hi[c] = 0;
             if (c_hi[c] > c_lo[c]) { in_lo = max(in_lo, c_lo[c]); in_hi = min(in_hi, c_hi[c]); }
             slope2[c] = p.slopes ? p.slopes[h] * kLog2e : 0.f;
+            ref[c] = p.slopes && c_hi[c] > 0 ? scored_ref(p, b, kh, c_hi[c]) : 0;
             const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + (size_t)row * p.ldq + h * HD;
 #pragma unroll
             for (int s = 0; s < NSTEP; ++s) {
@@ -335,7 +338,7 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int kp = KP ? kpos[KP ? e >> 2 : 0][e & 3] : vwin + e;
-                        sv[e] = __builtin_fmaf(slope2[c], (float)(kp - ref), sv[e]);
+                        sv[e] = __builtin_fmaf(slope2[c], (float)(kp - ref[c]), sv[e]);
                     }
                 }
                 float mx = NEG_BIG;
@@ -446,7 +449,7 @@ __global__ __launch_bounds__((NT == 1 && (INT8 || HD == 64) ? 512 : 256)) void s
                     const int rl = col / p.G, row = base + rl, h = kh * p.G + (col - rl * p.G);
                     int a, e;
                     scored_interval(p, row, a, e);
-                    scored_store<BF>(p, row, h, HD, d0, acc, mstar, l, e > a, ref);
+                    scored_store<BF>(p, row, h, HD, d0, acc, mstar, l, e > a, lse_ref(p, b, kh, d0, e));
                     if (p.ml_all && d0 == 0) *reinterpret_cast<float2*>(p.ml_all + (pair * p.ncol + col) * 2) = make_float2(mstar, l);
                 } else {
                     *reinterpret_cast<f32x4*>(p.tmp_out + (slot * p.ncol + col) * HD + d0) = acc;
@@ -529,7 +532,7 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
         }
         int a, e;
         scored_interval(p, row, a, e);
-        scored_store<BF>(p, row, h, HD, d0, acc, mn, l, e > a, p.slopes && e > a ? scored_ref(p, b, kh, mt.w) : 0);
+        scored_store<BF>(p, row, h, HD, d0, acc, mn, l, e > a, lse_ref(p, b, kh, d0, e));
         return;
     }
     // ---- weights: SL slots a thread, the first scores asked for before the columns' maxima and sums are merged
@@ -673,6 +676,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
     u32x4 qf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + (size_t)row * p.ldq + h * HD + s * 16 + half * 8);
+    const int ref = FORM == FORM_BIAS && seen ? scored_ref(p, b, kh, hi) : 0;
     const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;
     int idv = 0;                                    // block ids of 16 steps' units of 16 keys, a lane each
     auto ids_of = [&](int t0, int last) {
@@ -730,7 +734,6 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
     const int all = (khi - klo + 63) / 64, s1 = (int)((long)all * (part + 1) / p.parts);           // this part's steps
     s0 = (int)((long)all * part / p.parts);
     last16 = khi > 0 ? (khi - 1) & ~15 : 0;
-    const int ref = FORM == FORM_BIAS && khi > 0 ? __builtin_amdgcn_readfirstlane(scored_ref(p, b, kh, khi)) : 0;
     const float slope2 = FORM == FORM_BIAS ? p.slopes[h] * kLog2e : 0.f;
     f32x16 o[NDB];
 #pragma unroll

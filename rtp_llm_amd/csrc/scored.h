@@ -45,8 +45,9 @@ __device__ __forceinline__ int scored_block(const ScoredParams& p, const int32_t
     return min(max(bt[(int)(((unsigned long long)(unsigned)t * p.page_magic) >> 32)], 0), p.num_blocks - 1);
 }
 
-// The position that biases are taken from inside a sequence and head: that of its last seen slot, the newest token's as a rule.  Scores so stay small next to the keys that matter, however
-// far a row's position is; the log-sum-exp gets the rest, slope (reference - row position), at the end.
+// The position that a row's biases are taken from: that of its last seen slot, the newest token's as a rule.  Scores so stay small next to the keys that matter, however far the row's
+// position is; the log-sum-exp gets the rest, slope (reference - row position), at the end.  A row's own: with one for all rows of a sequence or tile, those that see slots far from it lose what
+// the bias between rounds away (slope 0.5, 60000 slots: 2e-3 of a weight).
 __device__ __forceinline__ int scored_ref(const ScoredParams& p, int b, int kh, int hi) {
     if (!p.key_pos) return hi - 1;
     const int blk = scored_block(p, p.block_table + (size_t)b * p.max_blocks, hi - 1);

@@ -1,4 +1,4 @@
-"""Edges of scored attention, tracked writes and eviction: scores that are all -inf."""
+"""Edges of scored attention, tracked writes and eviction: scores that are all -inf, rows whose intervals lie far apart under distance biases."""
 import pytest
 import torch
 
@@ -45,3 +45,38 @@ def test_scores_that_are_all_minus_infinity(nh, nkv, hd, dtype, int8, rows):
     assert bool(torch.isnan(got[:, 20:24]).all())
     t_w = weight_bound(want, 0.5, float(rel.max()), rows * nh // nkv, rows)
     assert bool(((got[:, others] - 0.5 - want).abs() <= t_w).all())
+
+
+@pytest.mark.parametrize("dtype,int8", TYPES)
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("nh,nkv,rows,gap", [(2, 1, 2, 60000), (4, 1, 8, 60000), (4, 1, 40, 60000), (1, 1, 24, 50000)])
+def test_biases_of_rows_that_see_slots_far_apart(nh, nkv, rows, gap, dtype, int8, planes):
+    """One half of a sequence's rows sees 40 slots at its start, the other half 40 a long way behind, both next to the rows' positions: biases are small in every row, and scores as exact as those of either
+    half alone."""
+    hd, page = 64, 64
+    n = gap + 40
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    kv, sc, bt, dense = make_cache([n], nkv, hd, page, dtype, int8, g, DEV)
+    q = torch.randn(rows, nh, hd, device=DEV, generator=g).to(dtype)
+    late = torch.arange(rows, device=DEV) % 2 == 1
+    begin, end = torch.where(late, gap, 0).int(), torch.where(late, n, 40).int()
+    positions, slopes = end + 2, torch.tensor([0.5 ** (1 + h) for h in range(nh)], device=DEV)
+    key_pos = None
+    if planes:                                                                # the slots' numbers, kept beside the cache
+        key_pos = torch.zeros(kv.shape[0], nkv, page, dtype=torch.int32, device=DEV)
+        key_pos[bt[0].long()] = torch.arange(bt.shape[1] * page, device=DEV).int().view(-1, 1, page).expand(-1, nkv, -1)
+    w = torch.zeros(kv.shape[0], nkv, page, device=DEV)
+    out, lse = ops.paged_attention_scored(q, kv, sc, bt, end, nkv, page, bt.shape[1] * page, begin=begin, q_len=rows, slopes=slopes, positions=positions, key_pos=key_pos, weights=w, decay=0.0,
+                                          return_lse=True)
+    out, got = out.view(rows, nh, hd).double(), gather_plane(w, bt, 0, n).double()
+    for half, first in ((~late, 0), (late, gap)):
+        k, v = (x[:, first:first + 40].contiguous() for x in dense[0])
+        m = int(half.sum())
+        ref, ref_lse, want, pv, size = attend(q[half], k, v, torch.zeros(m, device=DEV), torch.full((m,), 40, device=DEV), scale=hd ** -0.5, slopes=slopes, positions=positions[half] - first)
+        t_out, t_lse, rel = bounds(dtype, hd, 40, pv, size, ref)
+        assert bool(((out[half] - ref).abs() <= t_out).all()), float(((out[half] - ref).abs() / t_out).max())
+        diff = (lse[half].double() - ref_lse).abs()
+        assert bool((diff <= t_lse + 2.0 ** -22 * ref_lse.abs()).all()), float(diff.max())
+        t_w = weight_bound(want, 0.0, float(rel.max()), m * nh // nkv, rows)
+        assert bool(((got[:, first:first + 40] - want).abs() <= t_w).all()), float(((got[:, first:first + 40] - want).abs() / t_w).max())
+    assert bool((got[:, 40:gap] == 0).all())
