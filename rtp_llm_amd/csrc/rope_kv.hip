@@ -42,7 +42,8 @@ template <bool SLOTS> __device__ __forceinline__ RopePlace<SLOTS> rope_place(con
     r.pos_in = p.positions[t];
     r.seq = p.row_seq ? p.row_seq[t] : t / p.q_len;
     if constexpr (SLOTS) {
-        r.pos = min(max(r.pos_in, 0), p.max_pos - 1);
+        r.pos = max(r.pos_in, 0);
+        if (p.cos_sin) r.pos = min(r.pos, p.max_pos - 1);  // without a rotation every position from 0 on is kept
         r.slot_in = p.slots[t];
         r.slot = min(max(r.slot_in, 0), p.max_blocks * p.page - 1);
         if ((unsigned)r.seq >= (unsigned)p.nseq) { r.seq = 0; if (r.slot_in >= 0) r.slot_in = 0x7fffffff; }   // no such sequence: as a slot out of range

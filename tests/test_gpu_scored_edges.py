@@ -1,4 +1,4 @@
-"""Edges of scored attention, tracked writes and eviction: scores that are all -inf, rows whose intervals lie far apart under distance biases."""
+"""Edges of scored attention, tracked writes and eviction: scores that are all -inf, rows whose intervals lie far apart under distance biases, the largest position."""
 import pytest
 import torch
 
@@ -80,3 +80,24 @@ def test_biases_of_rows_that_see_slots_far_apart(nh, nkv, rows, gap, dtype, int8
         t_w = weight_bound(want, 0.0, float(rel.max()), m * nh // nkv, rows)
         assert bool(((got[:, first:first + 40] - want).abs() <= t_w).all()), float(((got[:, first:first + 40] - want).abs() / t_w).max())
     assert bool((got[:, 40:gap] == 0).all())
+
+
+@pytest.mark.parametrize("dtype,int8", TYPES)
+@pytest.mark.parametrize("T", [1, 70])
+def test_unrotated_rows_take_every_position(T, dtype, int8):
+    """Without a rotation any position from 0 to 2^31 - 1 is kept with its row; below 0 a row is out of range."""
+    nh, nkv, hd, page = 4, 2, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(T)
+    M = -(-T // page)
+    qkv = torch.randn(T, (nh + 2 * nkv) * hd, device=DEV, generator=g).to(dtype)
+    bt, slots = torch.arange(M, dtype=torch.int32, device=DEV).view(1, M), torch.arange(T, dtype=torch.int32, device=DEV)
+    for p, lost in (((1 << 31) - 1, 0), ((1 << 31) - 2, 0), (0, 0), (-1, T), (-(1 << 31), T)):
+        kv = torch.zeros(M, 2, nkv, page, hd, device=DEV, dtype=torch.int8 if int8 else dtype)
+        sc = torch.zeros(M, 2, nkv, page, device=DEV) if int8 else None
+        pos, w, oob = torch.full((M, nkv, page), 7, dtype=torch.int32, device=DEV), torch.ones(M, nkv, page, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+        ops.rope_kv_write_slots(qkv, None, None, torch.full((T,), p, dtype=torch.int32, device=DEV), slots, bt, kv, sc, nh, nkv, hd, page, q_len=T, key_pos=pos, weights=w, oob_count=oob)
+        assert int(oob) == lost, p
+        kept, cap = gather_plane(pos, bt, 0, M * page), M * page
+        assert bool((kept[:, :T] == (7 if lost else p)).all()) and bool((kept[:, T:] == 7).all()), p
+        assert bool((gather_plane(w, bt, 0, cap)[:, :T] == (1 if lost else 0)).all())
+        assert bool((kv != 0).any()) == (not lost)
