@@ -107,7 +107,9 @@ inline int scored_params(ScoredParams& p, const void* q, int ldq, const mi355_kv
                          int rows, int nh, const mi355_attn_score_t* sc, int max_seq, void* out, float* lse, float* weights, float decay) {
     MI355_CHECK_ARG(q && kv && kv->kv_base && block_table && sc && sc->end && out, "paged_attn_scored: null pointer");
     MI355_CHECK_ARG(kv->hd == 64 || kv->hd == 128, "paged_attn_scored: hd=%d (64 or 128)", kv->hd);
-    MI355_CHECK_ARG(kv->page >= 16 && kv->page % 16 == 0, "paged_attn_scored: page=%d (a multiple of 16)", kv->page);
+    // offsets inside a page's keys or values of one head are 32 bits
+    MI355_CHECK_ARG(kv->page >= 16 && kv->page % 16 == 0 && (long)kv->page * kv->hd * (kv->kv_dtype == MI355_KV_INT8 ? 1 : 2) < (1l << 31),
+                    "paged_attn_scored: page=%d (a multiple of 16, heads of %d below 2^31 bytes)", kv->page, kv->hd);
     MI355_CHECK_ARG(B > 0 && q_len > 0 && rows > 0 && nh > 0 && kv->nkv > 0 && nh % kv->nkv == 0, "paged_attn_scored: B=%d q_len=%d rows=%d nh=%d nkv=%d", B, q_len, rows, nh, kv->nkv);
     MI355_CHECK_ARG(row_start ? (long)rows <= (long)B * q_len : (long)rows == (long)B * q_len, "paged_attn_scored: %d rows, %d sequences of %s%d", rows, B, row_start ? "at most " : "", q_len);
     MI355_CHECK_ARG(B <= 65535 && kv->nkv <= 65535 && (long)rows * nh < (1l << 31) && (long)q_len * nh < (1l << 30), "paged_attn_scored: B=%d nkv=%d rows=%d nh=%d exceed the grid", B, kv->nkv, rows, nh);
