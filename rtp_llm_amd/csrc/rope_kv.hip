@@ -324,6 +324,7 @@ extern "C" int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void
     MI355_CHECK_ARG(qkv && slots && kv, "rope_kv_write_slots: null pointer");
     MI355_CHECK_ARG(nseq > 0 && q_len > 0 && (row_seq ? q_len == 1 : (long)nseq * q_len == T), "rope_kv_write_slots: %d rows, %d sequences, q_len=%d (1 where the rows' sequences are given)", T, nseq, q_len);
     MI355_CHECK_ARG((long)max_blocks_per_seq * kv->page < (1l << 31), "rope_kv_write_slots: %d blocks of %d tokens a sequence", max_blocks_per_seq, kv->page);
+    MI355_CHECK_ARG((long)kv->page * kv->hd < (1l << 31), "rope_kv_write_slots: page=%d (heads of %d below 2^31 values)", kv->page, kv->hd);
     return launch_rope<true>(qkv, nullptr, 0, ld, qkv_bias, cos_sin, kv->hd, cos_sin ? max_pos : 0x7fffffff, positions, row_seq, block_table, max_blocks_per_seq, T, q_len, nh, kv,
                              q_out, oob_count, RopeSlots{slots, nseq, key_pos, weights}, stream);
 }
