@@ -157,6 +157,10 @@ class Mi355ScoredDecodeImpl(Mi355PagedDecodeImpl):
         """Behind forward() of a step: sequences over the budget go back to it, in this layer.  -> the lengths (int32 [B], the same for every layer); the next step's sequence_lengths, with
         token_positions one above this step's."""
         c = self.cfg
+        if c.kv_budget <= 0:
+            raise ValueError("evict() is for a cache with a budget (kv_budget)")
+        if kv_cache.weights is None or kv_cache.key_pos is None:
+            raise ValueError("a cache with a budget needs its planes (kvcache.alloc_planes)")
         kv = kv_cache.kv_cache_base
         page = kv_cache.seq_size_per_block or kv.shape[3]
         return ops.kv_evict(kv_cache.weights, kv_cache.key_pos, self.block_table, self.seq_lens, self.positions + 1, kv.view(-1, 2, c.kv_head_num, page, c.size_per_head),

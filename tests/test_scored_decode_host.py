@@ -59,3 +59,13 @@ def test_rotated_models_need_the_rotation(monkeypatch):
         calls = []
         impl_of(monkeypatch, calls, table_blocks=4, lens=lens, **cfg).forward(torch.zeros(1, (NH + 2 * NKV) * HD, dtype=torch.float16), cache())
         assert calls[0][1] is None
+
+
+def test_eviction_needs_planes_and_a_budget(monkeypatch):
+    lens = torch.tensor([3])
+    impl = impl_of(monkeypatch, [], table_blocks=4, lens=lens, kv_budget=40)
+    with pytest.raises(ValueError, match="planes"):
+        impl.evict(cache(planes=False))
+    impl = impl_of(monkeypatch, [], table_blocks=4, lens=lens, softcap=30.0)
+    with pytest.raises(ValueError, match="budget"):
+        impl.evict(cache())
