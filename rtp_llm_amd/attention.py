@@ -35,7 +35,7 @@ class AttentionConfigs:       # cpp/model_utils/AttentionConfig.h:24-85 (per-ran
 
     @property
     def scored(self) -> bool:
-        return self.softcap > 0 or self.slopes is not None or self.kv_budget > 0
+        return self.softcap != 0 or self.slopes is not None or self.kv_budget != 0
 
 
 @dataclass
@@ -118,6 +118,10 @@ class Mi355ScoredDecodeImpl(Mi355PagedDecodeImpl):
     draws, and evict() brings the cache back to the budget."""
 
     def __init__(self, attn_configs: AttentionConfigs, attn_inputs: PyAttentionInputs, parallelism_config=None, cos_sin: Optional[torch.Tensor] = None, qkv_bias: Optional[torch.Tensor] = None):
+        if not attn_configs.softcap >= 0:
+            raise ValueError(f"softcap={attn_configs.softcap} (0: none, or above)")
+        if attn_configs.kv_budget < 0:
+            raise ValueError(f"kv_budget={attn_configs.kv_budget} (0: none, or above)")
         # no table means no rotation to the writer: that has to be the model's choice (slopes, or no rotated channels)
         if attn_configs.slopes is None and attn_configs.rope_dim != 0 and cos_sin is None:
             raise ValueError(f"rope_dim={attn_configs.rope_dim} needs cos_sin (models with slopes do not rotate)")

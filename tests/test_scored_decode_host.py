@@ -69,3 +69,10 @@ def test_eviction_needs_planes_and_a_budget(monkeypatch):
     impl = impl_of(monkeypatch, [], table_blocks=4, lens=lens, softcap=30.0)
     with pytest.raises(ValueError, match="budget"):
         impl.evict(cache())
+
+
+@pytest.mark.parametrize("cfg,said", [(dict(softcap=-30.0), "softcap"), (dict(kv_budget=-1), "kv_budget"), (dict(softcap=float("nan")), "softcap"), (dict(softcap=30.0, kv_budget=-1), "kv_budget")])
+def test_forms_that_are_none_are_refused(monkeypatch, cfg, said):
+    """A cap or a budget below zero is no plain configuration: it is refused, not left out."""
+    with pytest.raises(ValueError, match=said):
+        impl_of(monkeypatch, [], table_blocks=4, lens=torch.tensor([3]), **cfg)
