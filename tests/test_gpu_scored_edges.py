@@ -1,9 +1,11 @@
-"""Edges of scored attention, tracked writes and eviction: scores that are all -inf, rows whose intervals lie far apart under distance biases, the largest position."""
+"""Edges of scored attention, tracked writes and eviction: scores that are all -inf, rows whose intervals lie far apart under distance biases, the largest position, blocks outside the pool."""
 import pytest
 import torch
 
 from rtp_llm_amd import ops
+from tests import test_gpu_scored_attn as scored_attn
 from tests.scored_util import attend, bounds, gather_plane, make_cache
+from tests.test_gpu_scored_attn import run_case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -101,3 +103,50 @@ def test_unrotated_rows_take_every_position(T, dtype, int8):
         assert bool((kept[:, :T] == (7 if lost else p)).all()) and bool((kept[:, T:] == 7).all()), p
         assert bool((gather_plane(w, bt, 0, cap)[:, :T] == (1 if lost else 0)).all())
         assert bool((kv != 0).any()) == (not lost)
+
+
+@pytest.mark.parametrize("rows,nh", [(1, 4), (6, 4), (40, 4), (700, 4)])
+@pytest.mark.parametrize("int8", [False, True])
+def test_weights_of_blocks_outside_the_pool_are_not_written(rows, nh, int8):
+    """Ids that are no blocks read the pool's first or last block in place; no plane entry of those two, or of any block that the table does not name, changes.  700 rows: 1400 columns a head, whose
+    shares are added by a launch of their own."""
+    nkv, hd, page, nblk = 2, 64, 16, 12
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    if int8:
+        kv, sc = torch.randint(-128, 128, (nblk, 2, nkv, page, hd), generator=g, device=DEV, dtype=torch.int8), torch.rand(nblk, 2, nkv, page, device=DEV, generator=g) * 0.02
+    else:
+        kv, sc = torch.randn(nblk, 2, nkv, page, hd, device=DEV, generator=g).half(), None
+    bt = torch.tensor([[3, -7, 5, 1 << 30, 6], [-(1 << 31), 7, 12, 8, 9]], dtype=torch.int32, device=DEV)
+    w = torch.rand(nblk, nkv, page, device=DEV, generator=g)
+    before = w.clone()
+    q = torch.randn(2 * rows, nh, hd, device=DEV, generator=g).half()
+    end = torch.tensor([73] * rows + [80] * rows, dtype=torch.int32, device=DEV)
+    out = ops.paged_attention_scored(q, kv, sc, bt, end, nkv, page, 80, q_len=rows, weights=w)
+    assert bool(torch.isfinite(out.float()).all()) and bool(torch.isfinite(w).all())
+    named = [3, 5, 6, 7, 8, 9]
+    rest = [i for i in range(nblk) if i not in named]
+    assert torch.equal(w[rest], before[rest])
+    changed = w != before
+    assert bool(changed[[3, 5, 7, 8, 9]].all()) and bool(changed[6, :, :9].all()) and not bool(changed[6, :, 9:].any())
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("dtype,int8", TYPES)
+@pytest.mark.parametrize("cap,bias,mask", [(0.0, None, "causal"), (30.0, None, "window"), (0.0, "slots", "prefix"), (20.0, "planes", "causal"), (0.0, None, "documents")])
+def test_chunks_behind_long_contexts(nh, nkv, hd, dtype, int8, cap, bias, mask):
+    """A portion of a long prompt: more than 8192 slots, more than 128 columns a head, odd sizes."""
+    run_case(nh, nkv, hd, 16, dtype, int8, [8301, 250], [67, 33], mask, cap, bias, True, decay=0.5)
+
+
+@pytest.mark.parametrize("dtype,int8", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd,rows", [(28, 4, 128, 3), (28, 4, 128, 4), (14, 2, 64, 4), (16, 2, 128, 4)])
+@pytest.mark.parametrize("cap,bias,mask", [(0.0, "planes", "window"), (15.0, None, "causal")])
+def test_few_rows_in_two_tiles(monkeypatch, nh, nkv, hd, rows, dtype, int8, cap, bias, mask):
+    """17 to 32 columns a head, sequences of unequal length.
+    Random positions set scores hundreds apart: a row of two slots can draw 2^-133 of one beside a value of exactly 0.  What a product of a probability (and, 8 bits, a value's scale) has below 2^-126, the
+    smallest normal number of fp32 and bf16, may be 0: with codes up to 2^7, 16-bit values up to 2^3, at most 2^-119 a slot."""
+    def with_smallest(dtype, hd, L, pv, size, out):
+        t_out, t_lse, rel = bounds(dtype, hd, L, pv, size, out)
+        return t_out + L * 2.0 ** -119, t_lse, rel
+    monkeypatch.setattr(scored_attn, "bounds", with_smallest)
+    run_case(nh, nkv, hd, 32, dtype, int8, [500, 0, 77, 1200], [rows, rows - 1, 1, rows], mask, cap, bias, True)
