@@ -60,7 +60,7 @@ __device__ __forceinline__ float scored_decayed(const ScoredParams& p, float old
     return p.decay == 0.f ? sum : __builtin_fmaf(old, p.decay, sum);
 }
 
-// tanh.  Up to 0.625 a polynomial (u + u z P(z), z = u^2, P the minimax fit of degree 4 to (tanh(u) / u - 1) / z: 4.4e-9 relative), beyond (1 - t) / (1 + t) with
+// tanh.  Up to 0.625 a polynomial (u + u z P(z), z = u^2, P of degree 4 fitted to (tanh(u) / u - 1) / z: with its coefficients in fp32 8.6e-9 relative at worst), beyond (1 - t) / (1 + t) with
 // t = exp(-2 |u|).  The quotient alone loses, next to 0, what a cap of 50 multiplies: 3e-6 of a score of 5, and of its weight.  Scores far below their cap are the common ones,
 // and the polynomial is 7 full-rate instructions where the quotient takes two quarter-rate ones more: a wave forms the quotient only if one of its scores needs it.
 constexpr float kTanhNear = 0.625f;
