@@ -1245,6 +1245,7 @@ struct Plan {
     int    waves, tiles, parts, splits;                          // the many-row kernels
     size_t tmp_out, tmp_ml, ml_all, spill, meta, bytes;          // offsets; bytes: all
 };
+constexpr long GRID_THREADS = 1l << 32;   // a launch's threads along x are 32 bits
 constexpr int RUNS = 256;      // one block of the few-row kernel a compute unit
 Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, bool track, bool int8) {
     Plan pl{};
@@ -1341,7 +1342,8 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
     char* ws = (char*)workspace;
     if (pl.few) {
         const long np = (long)B * kv->nkv;
-        MI355_CHECK_ARG(np * (pl.ncol + (long)cdiv(max_seq_len, 256)) < (1l << 31) && (!pl.runs || np * cdiv(max_seq_len, 32) < (1l << 30)),
+        MI355_CHECK_ARG(np * (pl.ncol + (long)cdiv(max_seq_len, 256)) < (1l << 31) && (!pl.runs || np * cdiv(max_seq_len, 32) < (1l << 30)) &&
+                            pl.nblocks * 512l < GRID_THREADS && ((np * pl.ncol + 3) / 4 + (weights ? np * cdiv(max_seq_len, 1024) : 0)) * 256 < GRID_THREADS,
                         "paged_attn_scored: %d sequences of %d slots and %d heads exceed the grid", B, max_seq_len, nh);
         p.nblocks = pl.nblocks; p.ncol = pl.ncol; p.ctx_pad = pl.ctx_pad; p.runs = pl.runs;
         p.meta = (int4*)(ws + pl.meta);
@@ -1375,7 +1377,7 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
     c.tmp_out = pl.parts > 1 ? (float*)(ws + pl.tmp_out) : nullptr; c.tmp_ml = pl.parts > 1 ? (float4*)(ws + pl.tmp_ml) : nullptr;
     c.cols = weights ? (Col*)(ws + pl.ml_all) : nullptr; c.shares = weights && pl.splits > 1 ? (float*)(ws + pl.spill) : nullptr;
     c.reach = c.shares ? (int*)(c.shares + (size_t)pl.splits * B * kv->nkv * max_seq_len) : nullptr;
-    MI355_CHECK_ARG((long)pl.tiles * B * kv->nkv * pl.parts < (1l << 31) && (long)cdiv(max_seq_len, 256) * kv->nkv * B * std::max(1, pl.splits) < (1l << 31) && (long)q_len * p.G * p.G < (1l << 32),
+    MI355_CHECK_ARG((long)pl.tiles * B * kv->nkv * pl.parts * 64 * pl.waves < GRID_THREADS && (!weights || (long)cdiv(max_seq_len, 256) * kv->nkv * B * pl.splits * 512 < GRID_THREADS) && (long)q_len * p.G * p.G < (1l << 32),
                     "paged_attn_scored: %d rows of %d heads in %d sequences of %d slots exceed the grid", rows, nh, B, max_seq_len);
     int crc;
 #define LB_(HD_) do { if (bf) crc = int8 ? launch_chunk<HD_, true, true>(c, pl, st) : launch_chunk<HD_, false, true>(c, pl, st); \
