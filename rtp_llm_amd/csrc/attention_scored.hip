@@ -712,12 +712,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scored_chunk_kernel(const ChunkPar
             unit_at(st, d / KU, ti, hk);
             const uint16_t* kb = (const uint16_t*)p.kv_base + (uint64_t)hk * head_elems;
             const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + buf * ST::BYTES + d * 1024);
-            uint32_t ko = koff;
-            if constexpr (KU > NW) {                // the rows differ from load to load
-                const int r = (d % KU) * (1024 / ROW) + lane / CK;
-                ko = (uint32_t)(r * ROW + (((lane % CK) ^ swizzle_of<CK>(r)) << 4));
-            }
-            dma16(to, ko, kb + (uint32_t)(ti * HD));
+            dma16(to, koff, kb + (uint32_t)(ti * HD));
             dma16(to + KB, voff, kb + (uint64_t)(uint32_t)p.nkv * head_elems + (uint32_t)ti + (uint32_t)(d % KU * 32) * (uint32_t)p.page);
         }
     };
@@ -1265,8 +1260,9 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
         const long cols = (long)q_len * G;
         // Four waves a block, two blocks a compute unit: one fills in while the other one starts, ends or waits.  us by eight / by four: 16 x 64 rows 13.0 / 10.5, 4 x 512 29 / 25, 32 x 512
         // 157 / 144, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 916 / 946) and
-        // where keys and values are widened on the way (333 rows behind 3001 47 / 60).
-        pl.waves = cols <= 64 ? 2 : cols <= 128 || (!int8 && max_seq < 8192) ? 4 : 8;
+        // where keys and values are widened on the way (333 rows behind 3001 47 / 60).  Two a block are no form: at 35 to 64 columns behind 1000 to 12000 slots they took 1.01 to 1.27 of four's time,
+        // 1.01 to 1.6 over 8 bits, where they spilled most.
+        pl.waves = cols <= 128 || (!int8 && max_seq < 8192) ? 4 : 8;
         pl.tiles = (int)((cols + 32 * pl.waves - 1) / (32 * pl.waves));
         const long blocks = (long)pl.tiles * B * nkv, room = 256 * 8 / pl.waves;
         pl.parts = (int)std::max(1l, std::min({room / std::max(1l, blocks), (max_seq + 255l) / 256, 64l}));
@@ -1300,8 +1296,7 @@ int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
         return rc;
     };
     const long blocks = (long)pl.tiles * c.B * c.nkv * pl.parts;
-    int rc = pl.waves == 2 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 2>, Stage<HD, INT8, 2>::LDS, 128, blocks)
-           : pl.waves == 4 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 4>, Stage<HD, INT8, 4>::LDS, 256, blocks)
+    int rc = pl.waves == 4 ? run(scored_chunk_kernel<HD, INT8, BF, FORM, 4>, Stage<HD, INT8, 4>::LDS, 256, blocks)
                            : run(scored_chunk_kernel<HD, INT8, BF, FORM, 8>, Stage<HD, INT8, 8>::LDS, 512, blocks);
     if (rc != MI355_OK) return rc;
     if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 1024 / HD - 1) / (1024 / HD))), dim3(256), 0, st, c);
