@@ -1038,7 +1038,7 @@ __global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) 
 // instructions, the exponentials first, take 53% of that time and products 30%.  (Products of the next 32 columns laid among the exponentials of the last ones: 181 us against 170 then, the
 // registers' copies took more.)
 template <int HD, bool INT8, bool BF, int FORM>
-__global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p, int key_tiles, int splits) {
+__global__ __launch_bounds__(512, 2) void scored_sums_kernel(const ChunkParams p, int splits) {
     constexpr int KS = HD / 16, ROW = HD * 2, CK = ROW / 16, QB = 128 * ROW, SB = QB + 4096, LOADS = QB / 1024, JL = LOADS / 8, NS = 3;
     extern __shared__ __attribute__((aligned(16))) char su_sm[];
     float* meet = reinterpret_cast<float*>(su_sm);                   // [256], over the columns when they are done
@@ -1301,8 +1301,7 @@ int launch_chunk(const ChunkParams& c, const Plan& pl, hipStream_t st) {
     if (rc != MI355_OK) return rc;
     if (pl.parts > 1) hipLaunchKernelGGL((scored_parts_kernel<HD, BF>), dim3((unsigned)(((long)c.rows * c.nh + 1024 / HD - 1) / (1024 / HD))), dim3(256), 0, st, c);
     if (c.weights) {
-        const int key_tiles = cdiv(c.max_seq, 256);
-        rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 3 * (128 * HD * 2 + 4096) + 16, 512, (long)key_tiles * c.nkv * c.B * pl.splits, key_tiles, pl.splits);
+        rc = run(scored_sums_kernel<HD, INT8, BF, FORM>, 3 * (128 * HD * 2 + 4096) + 16, 512, (long)cdiv(c.max_seq, 256) * c.nkv * c.B * pl.splits, pl.splits);
         if (rc == MI355_OK && pl.splits > 1) hipLaunchKernelGGL(scored_decay_kernel, dim3(cdiv(c.max_seq, 256), c.nkv, c.B), dim3(256), 0, st, c, pl.splits);
     }
     return rc;

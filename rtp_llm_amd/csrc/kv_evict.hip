@@ -25,7 +25,7 @@ struct EvictParams {
     int32_t*       count;    // [B][nkv] moves
     int32_t*       lists;    // [B][nkv][2][cap]: sources, holes
     int32_t*       first;    // [B][nkv][units + 1]: holes before each 64 slots below keep
-    int max_blocks, num_blocks, nkv, hd, page, max_seq, keep, sinks, recent, cap, units;
+    int max_blocks, num_blocks, nkv, page, max_seq, keep, sinks, recent, cap, units;
     uint32_t page_magic;     // 2^32 / page + 1: floor(t / page) = (t magic) >> 32 for t page < 2^32
     __device__ __forceinline__ int page_of(int t) const { return (int)(((unsigned long long)(unsigned)t * page_magic) >> 32); }
 };
@@ -296,7 +296,7 @@ extern "C" int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_
     }
     EvictParams p;
     p.kv_base = kv->kv_base; p.scale_base = kv->scale_base; p.weights = weights; p.key_pos = key_pos; p.block_table = block_table; p.seq_lens = seq_lens; p.next_pos = next_pos;
-    p.new_lens = new_lens; p.max_blocks = max_blocks_per_seq; p.num_blocks = kv->num_blocks; p.nkv = kv->nkv; p.hd = kv->hd; p.page = kv->page; p.max_seq = max_seq_len;
+    p.new_lens = new_lens; p.max_blocks = max_blocks_per_seq; p.num_blocks = kv->num_blocks; p.nkv = kv->nkv; p.page = kv->page; p.max_seq = max_seq_len;
     p.keep = keep; p.sinks = sinks; p.recent = recent; p.cap = evict_cap(keep, max_seq_len);
     p.page_magic = (uint32_t)((1ull << 32) / (unsigned)kv->page + 1);
     p.units = evict_units(keep, max_seq_len);
