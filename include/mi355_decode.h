@@ -408,12 +408,14 @@ int mi355_rope_kv_write_slots(const void* qkv, int32_t ld, const void* qkv_bias,
  *   the key position from key_pos, or the slot itself where that is null.  Row r sees the slots begin[r] .. end[r] - 1 of its sequence (begin null: from 0; end is clamped to
  *   max_seq_len): causal rows have end = slot + 1, a window begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = the document's
  *   first slot.  A row that sees nothing gets zeros and a log-sum-exp of -inf.  Block ids are clamped into the pool.  What a slot holds,
- *   infinities and NaN included, reaches the rows that see it and no others.  scale > 0; softcap 0 (none) or 1e-6 .. 1e6.
- *   Pages of whole 16 tokens.  q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows behind the last are left alone), or, row_start null,
+ *   infinities and NaN included, reaches the rows that see it and no others.  A row whose seen scores are all -inf (below -6e29 counts as that) is not a number, and so are the weights of what it
+ *   sees.  scale > 0; softcap 0 (none) or 1e-6 .. 1e6.  Probabilities (8-bit caches: times the values' scales) are rounded to the activations' type before the product with the values; all else is fp32.
+ *   Pages of whole 16 tokens.  q [rows][ldq >= nh hd]; sequence b has the rows row_start[b] .. row_start[b + 1] - 1 (device, at most q_len each; rows <= B q_len; rows behind the last are left alone), or, row_start null,
  *   b q_len .. and rows = B q_len.  out [rows][nh hd]; lse [rows][nh] (fp32, natural logarithm) or null.  Any number of heads per kv head.
  *   weights (plane, or null): for every slot below the largest end of its sequence's rows that see something, weights <- decay weights + the sum over the sequence's rows and the heads of the
  *   kv head of exp(s - lse) (decay 1: accumulated since the start; 0: the last call's alone, whatever was there; between: fading).
- *   workspace: as many bytes as mi355_paged_attn_scored_workspace_bytes says, on 16 bytes; calls that may overlap need their own. */
+ *   workspace: as many bytes as mi355_paged_attn_scored_workspace_bytes says, on 16 bytes; calls that may overlap need their own.  With weights and few rows it holds
+ *   their scores: 4 bytes a (row, head) and slot of max_seq_len, which bounds slots, not positions: a budget's table keeps it small. */
 typedef struct {
     float          scale, softcap;
     const float*   slopes;     /* dev [nh] or NULL */
@@ -431,7 +433,8 @@ int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_kv_layer_t* 
 /* mi355_kv_evict: every (sequence, kv head) with more than `keep` tokens keeps `keep` of them: those at positions < sinks or >= next_pos[b] - recent first (sinks + recent <= keep),
  *   then the ones with the largest weights, the lower slot where weights are equal (NaN counts as the smallest).  Kept tokens in slots below `keep` stay where they are; the i-th of those
  *   behind moves into the i-th slot that an evicted token leaves: keys, values, scales, weights and positions.  What lies in slots >= keep afterwards is unspecified but still the pool's.
- *   new_lens[b] = min(seq_lens[b], keep) (may be null or seq_lens).  seq_lens are clamped to [0, max_seq_len]; tokens in blocks outside the pool are the first to go and never moved.
+ *   new_lens[b] = min(seq_lens[b], keep) (may be null or seq_lens).  seq_lens are clamped to [0, max_seq_len]; tokens in blocks outside the pool are the first to go and never
+ *   moved, and a token whose hole lies in one is lost.
  *   The caller appends at slot new_lens[b] and may free the pages behind it. */
 size_t mi355_kv_evict_workspace_bytes(int32_t B, int32_t nkv, int32_t keep, int32_t max_seq_len);
 int mi355_kv_evict(const mi355_kv_layer_t* kv, float* weights, int32_t* key_pos, const int32_t* block_table, int32_t max_blocks_per_seq, const int32_t* seq_lens,

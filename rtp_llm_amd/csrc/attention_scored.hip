@@ -7,6 +7,10 @@
 //
 // Everything is kept in the log2 domain: s2 = s log2(e), p = exp2(s2 - m) / l with m a column's running maximum and l its sum.  The weights are formed from m and l, not from their
 // logarithm: under distance biases of thousands that alone would be off by 5e-4 of a weight.
+//
+// Roundings to 16 bits, by choice: a probability (8-bit caches: times its value's scale, an fp32 number) to the activations' type before the second product, since matrix instructions that take
+// fp32 run at a sixteenth of the rate, and results.  Scores, maxima, sums, weights, parts and log-sum-exps stay fp32.  Relative errors of outputs against 64 bits, as computed in fp32 and rounded
+// once / here: 8 x 512 rows in fp16 2.07e-4 / 2.33e-4, 333 rows over 8 bits 2.07e-4 / 2.6e-4, documents in bf16 1.65e-3 / 1.81e-3.
 #include <algorithm>
 #include <type_traits>
 
@@ -56,7 +60,8 @@ __device__ __forceinline__ u32x4 seen_big(int t, int lo, int hi) {
 // Work: the tokens that any row of a sequence sees, in units of a group of 32 for each of a block's waves, times key/value heads, laid end to end over all sequences and dealt to the
 // blocks in equal runs.  A pair of a sequence and a head that lies inside one run is finished there, others leave a part in each run and scored_join_kernel merges them.  Sequences
 // of unequal length so take the time of their mean: a run may end one pair and begin the next.
-// Bound by memory: 64 sequences of up to 1024 tokens (28 over 4 heads of 128, 80 MB) 21 us, 3.7 TB/s, where a sum over a large array reads 4.0; one row over one short sequence is latency, 7 us.
+// Bound by memory: 64 sequences of up to 1024 tokens (28 over 4 heads of 128, 80 MB) 22 us, 3.6 TB/s, where a sum over a large array reads 4.0; one row over one short sequence is latency, 7 us.
+// Two to four rows a sequence, 64 sequences of 1000 (131 MB), with the join: 32 and 38 us, 4 tracked ones 54, over 8 bits 33.
 struct DecodeParams : ScoredParams {
     float*   tmp_out;    // [2 nblocks][ncol][hd]: parts; a run's first segment in slot 2 run, a later one that goes on in the next run in 2 run + 1
     float*   tmp_ml;     // [2 nblocks][ncol][2]
@@ -101,7 +106,9 @@ template <bool BF> __device__ __forceinline__ u32x4 widen_codes(uint32_t lo, uin
 }
 
 // Waves of a block, LDS of a wave's stage (keys, values, and, EXTRA, 1 KB of scales and positions), stages.  What is in flight fills LDS either way; eight waves, two a SIMD, hide what a group's chain
-// of product, softmax and product leaves idle, where a stage is 8 KB or less and the registers of two tiles of columns are not in the way.
+// of product, softmax and product leaves idle, where a stage is 8 KB or less and the registers of two tiles of columns are not in the way.  us with the join by four / by eight, one row a sequence:
+// 8 bits, 28 over 4 heads of 128: 1 x 1000 slots 9.8 / 10.3, 13 x 4000 23.7 / 19.5, 64 x 1000 22.4 / 20.3, 4 x 30000 38.7 / 33.5; 16 bits, 14 over 2 of 64: 9.1 / 9.7, 14.1 / 13.4, 14.8 / 14.1,
+// 20.6 / 18.7.
 template <int HD, bool INT8, int NT, bool EXTRA> struct Ring {
     static constexpr int ES = INT8 ? 1 : 2, KB = 32 * HD * ES, LOADS = 2 * KB / 1024 + (EXTRA ? 1 : 0), STAGE = LOADS * 1024, NW = NT == 1 && (INT8 || HD == 64) ? 8 : 4;
     static constexpr int N = HD == 128 && !INT8 ? 2 : NW == 4 ? 4 : HD == 64 && INT8 ? 3 : 2, UNIT = 32 * NW;
@@ -607,8 +614,11 @@ __global__ __launch_bounds__(256) void scored_join_kernel(const DecodeParams p, 
 // 16 (i / 2) + 8 half + 4 (i & 1) + r for row 8 i + 4 half + r: what a lane then holds of its column are two runs of eight keys, the second product's operand as it stands.
 // Keys and values come 64 at a time through LDS for all waves: by DMA, two steps ahead of the products with one barrier a step (three stages), or, 8 bits, through registers, which widen them
 // once for all waves.  A key's 16-byte pieces are swizzled by its low bits, a channel's 16 tokens lie side by side: no bank conflicts in either product's reads.
-// 28 heads of 128: 2 x 2048 rows behind 2048 slots 227 us (0.79 PFLOP/s), 4096 behind 12288 916 us (0.92), 8 x 512 capped 47 us.  Products take 43% of the busy time of a compute unit in the
-// first of these, vector instructions 44%: what is left is waiting, of the two kinds for each other in a wave and at a step's barrier.
+// 28 heads of 128, a launch among its like: 2 x 2048 rows behind 2048 slots 213 us (0.85 PFLOP/s; 239 in a trace of single passes), 4096 behind 12288 895 (0.94), 8 x 512 capped 42 (47), biased 45.
+// Products take 43% of the busy time of a compute unit in the first of these, vector instructions 44%: what is left is waiting, of the two kinds for each other in a wave and at a step's barrier.  A
+// wave reads 32 KB of fragments a step for 32 columns: at 128 bytes a clock LDS would be as busy as the products at their full rate.
+// 8 bits: 2 x 2048 behind 2048 276 us, 8 x 512 44, 333 rows behind 3001 48 in 10 parts.  The codes that are held over the products cost heads of 128 registers: 2 to 12 are spilled with eight waves, 17
+// to 25 with four.
 // What the weights' pass needs of a column.
 struct Col { float m, inv, slope2; int ref, lo, hi, pad0, pad1; };
 static_assert(sizeof(Col) == 32, "two 16-byte loads");
@@ -1034,7 +1044,7 @@ __global__ __launch_bounds__(256) void scored_parts_kernel(const ChunkParams p) 
 // The weights of many rows: S^T once more, a wave's 64 keys in registers, the columns streaming by, and every column's maximum and sum known.  A block takes 256 keys, its 8 waves the two halves of
 // 128 columns at a time (three stages of DMA); a probability is added in the lane of its column, lanes and halves meet once at the end: no atomics, the same sums every time.  A block's
 // columns are those of the rows between the first and the last that see some of its keys; tiles that most rows see come first; where blocks are few the columns are dealt to `splits` blocks
-// and scored_decay_kernel adds their shares.  2 x 2048 rows of 28 heads behind 2048 slots: 169 us, 0.53 PFLOP/s of products; compute units are busy for 85% of it, vector
+// and scored_decay_kernel adds their shares.  2 x 2048 rows of 28 heads behind 2048 slots: 163 us, 0.55 PFLOP/s of products; compute units are busy for 85% of it, vector
 // instructions, the exponentials first, take 53% of that time and products 30%.  (Products of the next 32 columns laid among the exponentials of the last ones: 181 us against 170 then, the
 // registers' copies took more.)
 template <int HD, bool INT8, bool BF, int FORM>
@@ -1250,7 +1260,10 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
     pl.few = (long)q_len * G <= 32;
     if (pl.few) {
         const long pairs = (long)B * nkv;
-        pl.runs = pairs < 4 * RUNS;                              // beyond, pairs are many enough to even out by themselves, and nothing has to be merged
+        // Runs take the time of the mean length where a block per pair takes that of the longest, and pay for parts and their merge.  us by pairs / by runs, 28 over 4 heads of 128, 256 pairs: lengths
+        // spread evenly up to 1000 18.7 / 26.2, all of 500 17.7 / 18.5, one of 8000 among 500s 73.8 / 23.0; 1024 pairs: 71.4 / 81.2, 65.9 / 64.4, 106 / 59; 2048: 127 / 147, 123 / 121, 166 / 135.
+        // From 1024 pairs on, four blocks a compute unit, they even out by themselves well enough.
+        pl.runs = pairs < 4 * RUNS;
         pl.nblocks = pl.runs ? RUNS : (int)pairs;
         pl.ncol = q_len * G; pl.ctx_pad = (max_seq + 63) / 32 * 32 + 32;
         pl.meta = region(pairs * sizeof(int4));
@@ -1259,12 +1272,15 @@ Plan plan_of(int B, int q_len, int rows, int nh, int nkv, int hd, int max_seq, b
     } else {
         const long cols = (long)q_len * G;
         // Four waves a block, two blocks a compute unit: one fills in while the other one starts, ends or waits.  us by eight / by four: 16 x 64 rows 13.0 / 10.5, 4 x 512 29 / 25, 32 x 512
-        // 157 / 144, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 916 / 946) and
+        // 157 / 144, 8 x 512 and 2 x 2048 behind 2048 the same.  Eight, which fetch keys and values half as often, where walks are long (4096 rows behind 12288 slots 895 / 913) and
         // where keys and values are widened on the way (333 rows behind 3001 47 / 60).  Two a block are no form: at 35 to 64 columns behind 1000 to 12000 slots they took 1.01 to 1.27 of four's time,
-        // 1.01 to 1.6 over 8 bits, where they spilled most.
+        // 1.01 to 1.6 over 8 bits, where they spilled most.  Up to 128 columns, where eight would leave half a block idle, four / eight of 35 to 126 columns: 16 bits 13.4 to 32.0 / 13.3 to 29.2 (heads
+        // of 128, eight ahead behind 12000 slots and for 32 over 8 heads), 11.0 to 21.1 / 11.3 to 21.5 (64); 8 bits 19.8 to 40.2 / 18.6 to 43.6 (128, eight ahead but for 8 kv heads), 15.7 to 25.1 / 16.0 to 25.4 (64).
         pl.waves = cols <= 128 || (!int8 && max_seq < 8192) ? 4 : 8;
         pl.tiles = (int)((cols + 32 * pl.waves - 1) / (32 * pl.waves));
         const long blocks = (long)pl.tiles * B * nkv, room = 256 * 8 / pl.waves;
+        // Parts of at least 256 keys, 64 at most: us by 128 / 256 / 512 keys, 40 rows of 28 over 4 heads behind 1000 slots 15.4 / 16.2 / 18.4, behind 3001 22.5 / 19.0 / 21.9, of 8 over 1 15.1 / 16.3 / 20.9,
+        // over 8 bits behind 3001 25.9 / 26.7 / 35.5; by at most 16 / 32 / 64 / 128, 40 rows of 8 over 1 behind 32000 73 / 47 / 39 / 40.
         pl.parts = (int)std::max(1l, std::min({room / std::max(1l, blocks), (max_seq + 255l) / 256, 64l}));
         if (pl.parts > 1) { pl.tmp_out = region((size_t)pl.parts * rows * nh * hd * 4); pl.tmp_ml = region((size_t)pl.parts * rows * nh * 16); }
         if (track) {
@@ -1351,9 +1367,12 @@ extern "C" int mi355_paged_attn_scored(const void* q, int32_t ldq, const mi355_k
 #undef LN_
         if (lrc != MI355_OK) return lrc;
         MI355_CHECK_LAUNCH("scored_decode_kernel");
-        // four slots a thread, or one where that leaves less than two blocks a compute unit
+        // Four slots a thread, or one where that leaves less than two blocks a compute unit.  us by one / by four, 28 over 4 heads: 2 x 8000 slots (64 blocks of 1024) 17.6 / 18.3, 16 x 4000 (256)
+        // 38.3 / 38.9, 32 x 4000 (512) 70.1 / 67.9, 64 x 3000 (768) 102 / 100.
         const int pairs = B * kv->nkv, sl = (long)pairs * cdiv(max_seq_len, 1024) >= 512 ? 4 : 1, chunks = weights ? cdiv(max_seq_len, 256 * sl) : 0;
-        const bool wide = pairs < 64;                            // at least four runs a pair
+        // A column a block where a pair has four runs or more, else four: us by four / by one, one row: 8 pairs of 6000 slots 16.6 / 15.6, 16 19.1 / 18.6, 64 of 1000 14.4 / 14.3, 256 31.5 / 32.2; four
+        // rows of 1000 slots, whose 28 columns a pair fill the chip sooner: 8 13.3 / 13.1, 32 16.5 / 17.6, 128 25.0 / 27.9.
+        const bool wide = pairs < 64;
         const int joins = wide ? pairs * pl.ncol : cdiv(pairs * pl.ncol, 4);
         const dim3 grid(joins + pairs * chunks);
 #define LK_(HD_, BF_, SL_) do { if (wide) hipLaunchKernelGGL((scored_join_kernel<HD_, BF_, SL_, 1>), grid, dim3(256), 0, st, p, joins, chunks); \

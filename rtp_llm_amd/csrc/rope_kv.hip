@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256) void rope_kv_write_kernel(const RopeParams p) 
 // whose columns lie token by token in a page: through LDS, so that a store's lanes are 16 tokens of a column.  By a wave per row and head a value went out as 64 lines of 2 bytes, and the lines of
 // consecutive rows from eight L2s.  us by waves / here: 28 over 4 heads of 128, 4096 rows 31.7 / 15.9
 // (4.7 TB/s), 1055 10.5 / 6.6, 265 4.5 / 4.2; 14 over 2 of 64, 4096 15.7 / 6.1, 512 4.1 / 3.2; 32 over 32 of 64, 1055 25.8 / 8.6, 64 3.8 / 3.0.
+// 8-bit caches stay with a wave per row and head, which has the head's largest value for its scale at hand: 8 x 512 rows of 28 over 4 heads of 128 into slots 36 us, in 16 bits 17 here.
 constexpr int RP_ROWS = 16, RP_HEADS = 4;
 template <bool BF, int HD, bool SLOTS>
 __global__ __launch_bounds__(256) void rope_kv_prompt_kernel(const RopeParams p) {

@@ -812,14 +812,16 @@ def paged_attention_scored(q: torch.Tensor, kv_base: torch.Tensor, scale_base: O
                            max_seq_len: int, *, begin: Optional[torch.Tensor] = None, row_start: Optional[torch.Tensor] = None, q_len: int = 1, scale: Optional[float] = None,
                            softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, key_pos: Optional[torch.Tensor] = None,
                            weights: Optional[torch.Tensor] = None, decay: float = 1.0, return_lse: bool = False, out: Optional[torch.Tensor] = None):
-    """q [rows, nh, hd] over a paged cache (pages of whole 16 tokens), rows of sequence b: row_start[b] .. row_start[b + 1] - 1 (int32 [B + 1] on the device, at most q_len each; rows behind
-    the last are left alone), or q_len each without row_start.  A row sees the slots begin[row] .. end[row] - 1 of its sequence (int32; begin None: from 0): causal end = slot + 1, a window
+    """q [rows, nh, hd] over a paged cache (pages of whole 16 tokens), rows of sequence b: row_start[b] .. row_start[b + 1] - 1 (int32 [B + 1] on the device, at most q_len each, rows <= B q_len; rows
+    behind the last are left alone), or q_len each without row_start.  A row sees the slots begin[row] .. end[row] - 1 of its sequence (int32; begin None: from 0): causal end = slot + 1, a window
     begin = end - window, a prefix that all rows see end = max(slot + 1, prefix), packed documents begin = first slot of the row's document; a row that sees nothing gets zeros.
     Scores: softcap * tanh(scale q.k / softcap) for softcap > 0, plus slopes[h] * (key position - positions[row]) with slopes (fp32 [nh]), key positions from the plane key_pos
     (int32 [num_blocks, nkv, page]) or the slots themselves.
     weights (fp32 plane) <- decay * weights + the probabilities of the call's rows and of the heads of each kv head, for the slots below the largest end
     of each sequence's rows that see something; kv_evict ranks by it.  The pages of a sequence are its own then: of one that two share, additions may be lost.
-    scale > 0, softcap 0 or 1e-6 to 1e6.  What a slot holds, infinities and NaN included, reaches the rows that see it and no others.
+    scale > 0, softcap 0 or 1e-6 to 1e6.  What a slot holds, infinities and NaN included, reaches the rows that see it and no others; a row whose seen scores are all -inf is not a number, and so are the
+    weights of what it sees.  Probabilities (8-bit caches: times the values' scales) are rounded to q's type before the product with the values; all else is fp32.
+    max_seq_len bounds slots (a call with weights keeps 4 bytes a (row, head) and slot of it where rows are few), not positions.
     The rows of q may have any stride of whole 16-byte pieces.  -> out [rows, nh * hd], with return_lse (out, log-sum-exp fp32 [rows, nh], -inf for a row that sees nothing)."""
     w = "paged_attention_scored"
     if q.dtype not in ACT_DTYPES or q.dim() != 3:
@@ -853,7 +855,8 @@ def kv_evict(weights: torch.Tensor, key_pos: torch.Tensor, block_table: torch.Te
     """Brings the cache of every sequence with more than `keep` tokens back to `keep`, for each kv head on its own: tokens at positions below `sinks` and from next_pos[b] - recent on stay
     (sinks + recent <= keep), the others by their weight, the lower slot first where weights are equal.  Survivors behind slot keep - 1 move into the slots below that became free, with their
     scales, weights and positions; what the slots from `keep` on hold afterwards is unspecified.  weights, key_pos: planes [num_blocks, nkv, page]; kv_base [num_blocks, 2, nkv,
-    page, hd]; seq_lens, next_pos int32 [B] on the device; the pages of block_table are each sequence's own.  -> the new lengths (int32 [B]); the next token goes to that slot."""
+    page, hd]; seq_lens, next_pos int32 [B] on the device; the pages of block_table are each sequence's own.
+    max_seq_len: no length exceeds it (None: the table's width; up to 32768 the ranks are kept in LDS, so give it where the table is wider than that).  -> the new lengths (int32 [B]); the next token goes to that slot."""
     w = "kv_evict"
     if weights.dim() != 3 or kv_base.dim() != 5 or kv_base.shape[2:4] != weights.shape[1:]:
         raise _C.Mi355Error(f"{w}: weights {tuple(weights.shape)}, cache {tuple(kv_base.shape)} (planes [blocks, heads, page] of a cache [blocks, 2, heads, page, channels])")
