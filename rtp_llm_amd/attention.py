@@ -134,7 +134,9 @@ class Mi355ScoredDecodeImpl(Mi355PagedDecodeImpl):
 
     def prepare(self, attn_inputs: PyAttentionInputs):
         super().prepare(attn_inputs)
-        self.slots, given = self.positions, attn_inputs.token_positions
+        # prepare_cuda_graph writes into these: not into the caller's
+        own = lambda t, given: t.clone() if attn_inputs.is_cuda_graph and t.data_ptr() == given.data_ptr() else t
+        self.slots, self.block_table, given = own(self.positions, attn_inputs.sequence_lengths), own(self.block_table, attn_inputs.kv_cache_kernel_block_id_device), attn_inputs.token_positions
         self.positions = (self.slots if given is None else given.to(device=self.slots.device, dtype=torch.int32)).clone()
 
     def prepare_cuda_graph(self, attn_inputs: PyAttentionInputs):

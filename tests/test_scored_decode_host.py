@@ -8,7 +8,7 @@ from rtp_llm_amd import attention as A
 NH, NKV, HD, PAGE = 8, 2, 64, 16
 
 
-def impl_of(monkeypatch, calls, *, table_blocks, lens, positions=None, cos_sin=None, **cfg):
+def impl_of(monkeypatch, calls, *, table_blocks, lens, positions=None, cos_sin=None, graph=False, **cfg):
     """An implementation whose operators only note their arguments."""
     def write(qkv, bias, cos, pos, slots, *a, **kw):
         calls.append(("write", cos, pos.clone(), slots.clone(), kw))
@@ -24,7 +24,8 @@ def impl_of(monkeypatch, calls, *, table_blocks, lens, positions=None, cos_sin=N
 
     for name, f in (("rope_kv_write_slots", write), ("paged_attention_scored", attend), ("kv_evict", evict)):
         monkeypatch.setattr(A.ops, name, f)
-    inputs = A.PyAttentionInputs(sequence_lengths=lens, kv_cache_kernel_block_id_device=torch.zeros(len(lens), table_blocks, dtype=torch.int32), token_positions=positions)
+    inputs = A.PyAttentionInputs(sequence_lengths=lens, kv_cache_kernel_block_id_device=torch.zeros(len(lens), table_blocks, dtype=torch.int32), token_positions=positions,
+                                is_cuda_graph=graph)
     return A.AttnImplFactory.get_fmha_impl(A.AttentionConfigs(NH, NKV, HD, **cfg), inputs, cos_sin=cos_sin)
 
 
@@ -76,3 +77,17 @@ def test_forms_that_are_none_are_refused(monkeypatch, cfg, said):
     """A cap or a budget below zero is no plain configuration: it is refused, not left out."""
     with pytest.raises(ValueError, match=said):
         impl_of(monkeypatch, [], table_blocks=4, lens=torch.tensor([3]), **cfg)
+
+
+def test_refreshed_buffers_are_the_implementations_own(monkeypatch):
+    """prepare_cuda_graph refreshes buffers in place: not the lengths, positions and tables that the first inputs came with."""
+    calls = []
+    lens, positions = torch.tensor([3, 5], dtype=torch.int32), torch.tensor([30, 50], dtype=torch.int32)
+    impl = impl_of(monkeypatch, calls, table_blocks=4, lens=lens, positions=positions, graph=True, kv_budget=40)
+    table = impl.inputs.kv_cache_kernel_block_id_device
+    kept = [x.clone() for x in (lens, positions, table)]
+    at = [x.data_ptr() for x in (impl.slots, impl.positions, impl.seq_lens, impl.block_table)]
+    impl.prepare_cuda_graph(A.PyAttentionInputs(sequence_lengths=lens + 1, kv_cache_kernel_block_id_device=table + 7, token_positions=positions + 1))
+    assert [x.data_ptr() for x in (impl.slots, impl.positions, impl.seq_lens, impl.block_table)] == at
+    assert impl.slots.tolist() == [4, 6] and impl.positions.tolist() == [31, 51] and impl.seq_lens.tolist() == [5, 7] and bool((impl.block_table == 7).all())
+    assert all(torch.equal(a, b) for a, b in zip((lens, positions, table), kept))
